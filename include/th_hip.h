@@ -285,6 +285,135 @@ int64_t th_attention_decode_workspace_bytes(int32_t batch, int32_t heads_q, int3
 
 int th_attention_decode(const th_decode_desc* desc, void* stream);
 
+/* -------------------------------------------------------- rotary positions
+ * Every head of x [tokens, heads*head_dim] has its first rot_dim dims rotated
+ * in pairs (a, b) by the token's own position (no counterpart in the
+ * reference, which bakes one table of positions 0..S-1 into a GEMM,
+ * optimizer/param_transforms.py:47-51):
+ *   a' = scale (a cos phi - b sin phi),  b' = scale (b cos phi + a sin phi),  phi = position * freqs[i]
+ * pair i is dims (i, i + rot_dim/2), or (2i, 2i+1) with interleaved. Dims past
+ * rot_dim are copied. inverse takes -phi: with the same scale that is the
+ * gradient of the forward call. Angles are reduced in 64 bits, so positions
+ * may lie anywhere in their type. out may be x itself (same row stride).
+ */
+typedef struct th_rope_desc {
+  int64_t tokens;
+  int32_t heads, head_dim;   /* head_dim <= 1024 */
+  int32_t rot_dim;           /* even, 2..head_dim */
+  int32_t interleaved, inverse;
+  int32_t dtype;             /* TH_BF16 or TH_F32: x and out */
+  int32_t positions_dtype;   /* TH_I32 or TH_I64 */
+  float scale;
+  const void* x; int64_t ld_x;   /* row strides in elements (>= heads*head_dim) */
+  const void* positions;         /* [tokens] */
+  const double* freqs;           /* [rot_dim/2] radians per position */
+  void* out; int64_t ld_out;
+} th_rope_desc;
+
+int th_rope(const th_rope_desc* desc, void* stream);
+
+/* ------------------------------------------------------- paged KV cache
+ * A cache is [pages][page_size][heads_kv][head_dim] with its own page, token
+ * and head strides; row r of the page table lists the pages of sequence r in
+ * the order of its tokens. Token t of a call stands at positions[t] of row
+ * rows[t] (of row t when rows is NULL); positions[t] < 0 marks a padded
+ * token. No counterpart in the reference (no KV cache, models/llama_block.py:82-105).
+ *
+ * th_paged_append rotates the keys (th_rope's rotation; rot_dim 0: none) and
+ * stores keys and values at their slots, an e4m3 cache as e4m3(x / scale_h)
+ * saturated at +-448. With heads_q > 0 the queries are rotated into q_out in
+ * the same launch. A padded token is skipped: nothing of it is written. A
+ * token whose row, position or page lies outside the table or the cache is
+ * not stored and counted once in *n_invalid (if given; the caller zeroes it);
+ * its queries are rotated all the same. Two tokens of one call must not share
+ * a slot.
+ */
+typedef struct th_paged_append_desc {
+  int64_t tokens;
+  int32_t heads_q, heads_kv, head_dim;  /* head_dim <= 1024 */
+  int32_t rot_dim, interleaved;
+  int32_t in_dtype;                     /* TH_BF16 or TH_F32: q, k, v */
+  int32_t cache_dtype;                  /* TH_BF16 or TH_F8E4M3 */
+  int32_t page_size;                    /* tokens per page, a power of two */
+  int32_t n_rows, row_pages;            /* page table [n_rows][row_pages] */
+  int64_t pages;
+  float scale;                          /* of the rotation (cos and sin times this) */
+  int32_t pad_;
+  const int32_t* positions;             /* [tokens] */
+  const int32_t* rows;                  /* optional [tokens] */
+  const int32_t* page_table; int64_t ld_page_table;
+  const double* freqs;                  /* [rot_dim/2] */
+  const void* q; int64_t ld_q;          /* [tokens, heads_q*head_dim] */
+  void* q_out; int64_t ld_q_out;        /* bf16; may be q when q is bf16 (same row stride) */
+  const void* k; int64_t ld_k;          /* [tokens, heads_kv*head_dim] */
+  const void* v; int64_t ld_v;
+  void* k_cache; int64_t k_stride_page, k_stride_t, k_stride_h;  /* elements */
+  void* v_cache; int64_t v_stride_page, v_stride_t, v_stride_h;
+  const float* k_scale;                 /* optional [heads_kv], e4m3 caches only (default 1) */
+  const float* v_scale;
+  int32_t* n_invalid;
+} th_paged_append_desc;
+
+int th_paged_append(const th_paged_append_desc* desc, void* stream);
+
+/* One query per token against the pages of its row: token t with pos =
+ * positions[t] sees the keys j of its row with max(0, pos + 1 - window) <= j
+ * <= pos (all from 0 without a window),
+ *   s_j = scale q . k_j k_scale_h;  s_j = softcap tanh(s_j / softcap) when softcap > 0;
+ *   s_j -= slopes[h] (pos - j) when slopes is given;
+ *   o = sum_j softmax(s)_j v_j v_scale_h.
+ * Query head h reads kv head h / (heads_q / heads_kv). Keys past the table's
+ * end and keys in pages outside the cache are left out; a token that sees no
+ * key (padded, or of a row outside the table) gets zeros. What the slots of
+ * unseen keys hold, NaN included, does not reach the result. The keys of all
+ * tokens are dealt out evenly over the GPU, whatever the lengths, and the
+ * parts are joined through the workspace.
+ */
+typedef struct th_paged_attn_desc {
+  int32_t tokens, heads_q, heads_kv, head_dim;  /* head_dim 64 or 128 */
+  int32_t cache_dtype;                  /* TH_BF16 or TH_F8E4M3; q and o are bf16 */
+  int32_t page_size;                    /* a power of two, at least 16 */
+  int32_t n_rows, row_pages;
+  int64_t pages;
+  int32_t window;                       /* 0: none */
+  float scale, softcap;                 /* softcap 0: none */
+  int32_t pad_;
+  const int32_t* positions;             /* [tokens] */
+  const int32_t* rows;                  /* optional [tokens] */
+  const int32_t* page_table; int64_t ld_page_table;
+  const void* q; int64_t ld_q;          /* [tokens, heads_q*head_dim] */
+  const void* k_cache; int64_t k_stride_page, k_stride_t, k_stride_h;  /* elements */
+  const void* v_cache; int64_t v_stride_page, v_stride_t, v_stride_h;
+  const float* slopes;                  /* optional [heads_q] */
+  const float* k_scale;                 /* optional [heads_kv], e4m3 caches only (default 1) */
+  const float* v_scale;
+  void* o; int64_t ld_o;                /* [tokens, heads_q*head_dim] */
+  float* workspace; int64_t workspace_bytes;  /* 16-byte aligned; holds nothing between calls */
+} th_paged_attn_desc;
+
+/* Workspace th_paged_attention needs for these sizes on the current device (-1: bad sizes). */
+int64_t th_paged_attention_workspace_bytes(int32_t tokens, int32_t heads_q, int32_t heads_kv, int32_t head_dim);
+
+int th_paged_attention(const th_paged_attn_desc* desc, void* stream);
+
+/* Copies page src[i] onto page dst[i] of both caches in every layer, and, with
+ * a page table, renames its entries p in [0, pages) to page_map[p]. A pair
+ * with an index outside [0, pages) is skipped. No page may be both a source
+ * and a destination, or twice a destination (the copies run at once).
+ */
+typedef struct th_page_copy_desc {
+  int32_t layers, n;                    /* n pairs */
+  int64_t pages, page_bytes;            /* bytes of one page of one tensor (dense) */
+  void* k_cache; int64_t k_layer_bytes, k_page_bytes;  /* strides in bytes */
+  void* v_cache; int64_t v_layer_bytes, v_page_bytes;
+  const int32_t* src; const int32_t* dst;  /* [n] */
+  int32_t* page_table; int64_t ld_page_table;  /* optional [n_rows][row_pages] */
+  int32_t n_rows, row_pages;
+  const int32_t* page_map;              /* [pages], with page_table */
+} th_page_copy_desc;
+
+int th_page_copy(const th_page_copy_desc* desc, void* stream);
+
 /* ------------------------------------------------------------ SSD scan
  * The Mamba-2 scan, per (batch b, head h) over token-major operands:
  *   y_t = sum_{s<=t} (C_t . B_s) exp(cum_t - cum_s) dt_s x_s + D_h x_t  [* gate_t]

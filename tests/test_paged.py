@@ -1,0 +1,225 @@
+"""The rotary and paged-cache entry points on the CPU: struct layouts, frequencies, refusals.
+
+No call here reaches a device: each fails its argument checks, or stops where the library or the
+tensor's device is missing.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+import math
+import subprocess
+from pathlib import Path
+
+import pytest
+import torch
+
+REPO = Path(__file__).resolve().parents[1]
+HEADER = REPO / "include" / "th_hip.h"
+STRUCTS = {"th_rope_desc": "RopeDesc", "th_paged_append_desc": "PagedAppendDesc", "th_paged_attn_desc": "PagedAttnDesc",
+           "th_page_copy_desc": "PageCopyDesc"}
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from torch_helion.hip import abi
+
+    if not abi.library_path().exists():
+        pytest.skip("libth_hip.so not built (run __graft_entry__.build())")
+    return abi.load()
+
+
+def test_struct_layouts_match_the_header(tmp_path):
+    from torch_helion.hip import abi
+
+    lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "th_hip.h"', "int main(void){"]
+    for cname, pyname in STRUCTS.items():
+        lines.append(f'printf("{cname} size %zu\\n", sizeof({cname}));')
+        lines += [f'printf("{cname} {f} %zu\\n", offsetof({cname}, {f}));' for f, _ in getattr(abi, pyname)._fields_]
+    src, exe = tmp_path / "probe.c", tmp_path / "probe"
+    src.write_text("\n".join(lines + ["return 0;}"]))
+    subprocess.run(["gcc", "-I", str(HEADER.parent), str(src), "-o", str(exe)], check=True)
+    out = subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.splitlines()
+    got = {tuple(line.split()[:2]): int(line.split()[2]) for line in out}
+    for cname, pyname in STRUCTS.items():
+        st = getattr(abi, pyname)
+        assert got[(cname, "size")] == C.sizeof(st)
+        for f, _ in st._fields_:
+            assert got[(cname, f)] == getattr(st, f).offset, (cname, f)
+
+
+# ------------------------------------------------------------------ frequencies
+def test_rope_frequencies():
+    from torch_helion.hip import abi, ops
+
+    f = ops.rope_frequencies(8, 10000.0)
+    assert f.dtype == torch.float64 and torch.allclose(f, torch.tensor([1.0, 0.1, 0.01, 0.001], dtype=torch.float64), rtol=1e-15)
+    assert torch.allclose(ops.rope_frequencies(8, 10000.0, scaling="linear", factor=4.0), f / 4, rtol=1e-15)
+    ntk = ops.rope_frequencies(8, 10000.0, scaling="ntk", factor=4.0)
+    assert ntk[0] == 1.0 and math.isclose(ntk[-1], 0.001 / 4, rel_tol=1e-12)
+    parts = ops.rope_frequencies(128, 500000.0, scaling="by_parts", factor=8.0, original_len=8192, low=1.0, high=4.0)
+    plain = ops.rope_frequencies(128, 500000.0)
+    turns = plain * 8192 / (2 * math.pi)
+    assert torch.equal(parts[turns > 4], plain[turns > 4])
+    assert torch.allclose(parts[turns < 1], plain[turns < 1] / 8, rtol=1e-15)
+    mid = (turns > 1) & (turns < 4)
+    assert mid.any() and (parts[mid] < plain[mid]).all() and (parts[mid] > plain[mid] / 8).all()
+    for bad in (dict(rot_dim=7), dict(rot_dim=0), dict(scaling="other"), dict(scaling="by_parts"),
+                dict(scaling="linear", factor=0.0), dict(rot_dim=2, scaling="ntk", factor=2.0)):
+        with pytest.raises(abi.HipBackendError):
+            ops.rope_frequencies(**{"rot_dim": 8, "theta": 10000.0, **bad})
+
+
+# ------------------------------------------------------------------ refusals of the C entries
+def rope_desc(abi):
+    d = abi.RopeDesc()
+    d.tokens, d.heads, d.head_dim, d.rot_dim, d.dtype, d.positions_dtype, d.scale = 4, 2, 64, 64, abi.TH_BF16, abi.TH_I32, 1.0
+    d.x, d.ld_x, d.positions, d.freqs, d.out, d.ld_out = 4096, 128, 8192, 12288, 16384, 128
+    return d
+
+
+def append_desc(abi):
+    d = abi.PagedAppendDesc()
+    d.tokens, d.heads_q, d.heads_kv, d.head_dim, d.rot_dim = 4, 4, 2, 64, 64
+    d.in_dtype, d.cache_dtype, d.page_size, d.n_rows, d.row_pages, d.pages, d.scale = abi.TH_BF16, abi.TH_BF16, 16, 4, 2, 9, 1.0
+    d.positions, d.page_table, d.ld_page_table, d.freqs = 4096, 8192, 2, 12288
+    d.q, d.ld_q, d.q_out, d.ld_q_out, d.k, d.ld_k, d.v, d.ld_v = 16384, 256, 20480, 256, 24576, 128, 28672, 128
+    d.k_cache, d.k_stride_page, d.k_stride_t, d.k_stride_h = 32768, 2048, 128, 64
+    d.v_cache, d.v_stride_page, d.v_stride_t, d.v_stride_h = 65536, 2048, 128, 64
+    return d
+
+
+def attn_desc(abi):
+    d = abi.PagedAttnDesc()
+    d.tokens, d.heads_q, d.heads_kv, d.head_dim, d.cache_dtype, d.page_size = 4, 4, 2, 64, abi.TH_BF16, 16
+    d.n_rows, d.row_pages, d.pages, d.scale = 4, 2, 9, 0.125
+    d.positions, d.page_table, d.ld_page_table, d.q, d.ld_q, d.o, d.ld_o = 4096, 8192, 2, 16384, 256, 20480, 256
+    d.k_cache, d.k_stride_page, d.k_stride_t, d.k_stride_h = 32768, 2048, 128, 64
+    d.v_cache, d.v_stride_page, d.v_stride_t, d.v_stride_h = 65536, 2048, 128, 64
+    d.workspace, d.workspace_bytes = 131072, 1 << 40
+    return d
+
+
+def copy_desc(abi):
+    d = abi.PageCopyDesc()
+    d.layers, d.n, d.pages, d.page_bytes = 2, 3, 9, 4096
+    d.k_cache, d.k_layer_bytes, d.k_page_bytes = 4096, 65536, 4096
+    d.v_cache, d.v_layer_bytes, d.v_page_bytes = 262144, 65536, 4096
+    d.src, d.dst, d.page_table, d.ld_page_table, d.n_rows, d.row_pages, d.page_map = 8192, 8256, 12288, 2, 4, 2, 16384
+    return d
+
+
+REFUSED = [
+    ("th_rope", rope_desc, [
+        ({"rot_dim": 63}, "rot_dim"), ({"rot_dim": 66}, "rot_dim"), ({"rot_dim": 0}, "rot_dim"), ({"dtype": 2}, "dtype"),
+        ({"positions_dtype": 0}, "positions dtype"), ({"head_dim": 2048, "rot_dim": 64}, "head_dim"), ({"heads": 0}, "heads"),
+        ({"ld_x": 127}, "row stride"), ({"ld_out": 64}, "row stride"), ({"out": 4096, "ld_out": 256}, "in place"),
+        ({"freqs": 0}, "null"), ({"positions": 0}, "null"), ({"tokens": -1}, "tokens"), ({"tokens": 1 << 31}, "tokens")]),
+    ("th_paged_append", append_desc, [
+        ({"rot_dim": 5}, "rot_dim"), ({"rot_dim": 66}, "rot_dim"), ({"page_size": 24}, "page_size"), ({"page_size": 0}, "page_size"),
+        ({"cache_dtype": 0}, "cache_dtype"), ({"in_dtype": 3}, "in_dtype"), ({"heads_kv": 0}, "heads"), ({"heads_q": -1}, "heads"),
+        ({"n_rows": 0}, "page table"), ({"ld_page_table": 1}, "page table"), ({"pages": 0}, "page table"),
+        ({"ld_k": 64}, "row stride"), ({"ld_q": 64}, "row stride"), ({"q_out": 16384, "ld_q_out": 512}, "in place"),
+        ({"q_out": 16384, "in_dtype": 0}, "in place"), ({"k_stride_h": 32}, "cache stride"), ({"v_stride_t": 0}, "cache stride"),
+        ({"k_scale": 4096}, "e4m3"), ({"tokens": 5}, "exceed the table"), ({"freqs": 0}, "null"), ({"q": 0}, "null"),
+        ({"page_table": 0}, "null")]),
+    ("th_paged_attention", attn_desc, [
+        ({"heads_q": 5}, "multiple"), ({"head_dim": 96}, "head_dim"), ({"cache_dtype": 0}, "cache_dtype"), ({"page_size": 8}, "page_size"),
+        ({"page_size": 48}, "page_size"), ({"row_pages": 0}, "page table"), ({"window": -1}, "window"), ({"softcap": -1.0}, "softcap"),
+        ({"softcap": float("nan")}, "softcap"), ({"ld_q": 255}, "row strides"), ({"ld_q": 260}, "16 bytes"),
+        ({"k_stride_h": 68}, "16 bytes"), ({"v_stride_page": 2050}, "16 bytes"), ({"cache_dtype": 3, "k_stride_t": 136}, "16 bytes"),
+        ({"k_stride_t": 1 << 23}, "token strides"), ({"q": 16392}, "16-byte"), ({"v_cache": 65544}, "16-byte"), ({"v_scale": 4096}, "e4m3"),
+        ({"tokens": -1}, "tokens"), ({"tokens": 5}, "exceed the table"), ({"positions": 0}, "null"), ({"o": 0}, "null"),
+        ({"row_pages": 1 << 27, "ld_page_table": 1 << 27}, "2^31")]),
+    ("th_page_copy", copy_desc, [
+        ({"layers": 0}, "sizes"), ({"n": -1}, "sizes"), ({"page_bytes": 4104}, "16"), ({"k_cache": 4104}, "16"),
+        ({"k_page_bytes": 2048}, "page stride"), ({"v_layer_bytes": 0}, "layer stride"), ({"page_map": 0}, "page table"),
+        ({"ld_page_table": 1}, "page table"), ({"src": 0}, "null"), ({"n": 1 << 30, "page_bytes": 16}, "one launch")]),
+]
+
+
+@pytest.mark.parametrize("entry,make,over,message", [(e, m, o, s) for e, m, cases in REFUSED for o, s in cases])
+def test_refusals(lib, entry, make, over, message):
+    from torch_helion.hip import abi
+
+    d = make(abi)
+    for name, value in over.items():
+        setattr(d, name, value)
+    assert getattr(lib, entry)(C.byref(d), None) == abi.TH_ERR_INVALID
+    text = abi.last_error(lib)
+    assert text.startswith(entry) and message in text, text
+
+
+@pytest.mark.parametrize("entry,make,empty", [
+    ("th_rope", rope_desc, {"tokens": 0, "x": 0, "positions": 0}), ("th_paged_append", append_desc, {"tokens": 0, "k": 0}),
+    ("th_paged_attention", attn_desc, {"tokens": 0, "q": 0, "workspace": 0}),
+    ("th_page_copy", copy_desc, {"n": 0, "page_table": 0, "src": 0})])
+def test_null_empty_and_valid_descriptors(lib, entry, make, empty):
+    """A null descriptor is refused, an empty call is a no-op, a valid one passes every check (and stops at the
+    missing th_init where there is no GPU)."""
+    from torch_helion.hip import abi
+
+    fn = getattr(lib, entry)
+    assert fn(None, None) == abi.TH_ERR_INVALID
+    d = make(abi)
+    if not torch.cuda.is_available():
+        assert fn(C.byref(d), None) == abi.TH_ERR_NOT_INIT, abi.last_error(lib)
+    for name, value in empty.items():
+        setattr(d, name, value)
+    assert fn(C.byref(d), None) == abi.TH_OK, abi.last_error(lib)
+
+
+def test_workspace_query(lib):
+    for bad in ((-1, 8, 2, 64), (4, 0, 2, 64), (4, 8, 3, 64), (4, 8, 2, 96), (4, 8, 0, 64)):
+        assert lib.th_paged_attention_workspace_bytes(*bad) == -1
+    assert lib.th_paged_attention_workspace_bytes(4, 8, 2, 64) >= 0
+
+
+# ------------------------------------------------------------------ refusals of the Python layer
+def tensors():
+    t, hk, d = 4, 2, 64
+    kc = torch.zeros(9, 16, hk, d, dtype=torch.bfloat16)
+    return dict(k=torch.zeros(t, hk * d, dtype=torch.bfloat16), v=torch.zeros(t, hk * d, dtype=torch.bfloat16),
+                positions=torch.zeros(t, dtype=torch.int32), k_cache=kc, v_cache=torch.zeros_like(kc),
+                page_table=torch.zeros(t, 2, dtype=torch.int32), q=torch.zeros(t, 4 * d, dtype=torch.bfloat16),
+                out=torch.zeros(t, 4 * d, dtype=torch.bfloat16), freqs=torch.zeros(d // 2, dtype=torch.float64))
+
+
+@pytest.mark.parametrize("change,message", [
+    ({"positions": torch.zeros(4, dtype=torch.int64)}, "positions"), ({"positions": torch.zeros(3, dtype=torch.int32)}, "positions"),
+    ({"positions": torch.zeros(8, dtype=torch.int32)[::2]}, "positions"), ({"page_table": torch.zeros(4, 2)}, "page_table"),
+    ({"v_cache": torch.zeros(9, 16, 2, 32, dtype=torch.bfloat16)}, "caches"), ({"rows": torch.zeros(4, dtype=torch.int64)}, "rows"),
+    ({"k_cache": torch.zeros(9, 16, 64, 2, dtype=torch.bfloat16).transpose(2, 3)}, "contiguous"),
+    ({"k_scale": torch.ones(3)}, "k_scale"), ({}, "HIP device"),
+])
+def test_paged_argument_checks(change, message):
+    from torch_helion.hip import abi, ops
+
+    a = {**tensors(), **change}
+    rest = {n: a[n] for n in ("rows", "k_scale") if n in a}
+    with pytest.raises(abi.HipBackendError, match=message):
+        ops.paged_append(a["k"], a["v"], a["positions"], a["k_cache"], a["v_cache"], a["page_table"], freqs=a["freqs"], **rest)
+    with pytest.raises(abi.HipBackendError, match=message):
+        ops.paged_attention(a["q"], a["k_cache"], a["v_cache"], a["page_table"], a["positions"], a["out"], scale=1.0, **rest)
+
+
+def test_more_argument_checks():
+    from torch_helion.hip import abi, ops
+
+    a = tensors()
+    append = lambda **kw: ops.paged_append(**{**{n: a[n] for n in ("k", "v", "positions", "k_cache", "v_cache", "page_table")}, **kw})
+    attend = lambda **kw: ops.paged_attention(**{**{n: a[n] for n in ("q", "k_cache", "v_cache", "page_table", "positions", "out")},
+                                                 "scale": 1.0, **kw})
+    rope = lambda **kw: ops.rope(**{**dict(x=a["q"], positions=a["positions"], freqs=a["freqs"], out=a["out"], head_dim=64), **kw})
+    copy = lambda **kw: ops.copy_pages(**{**dict(k_cache=a["k_cache"], v_cache=a["v_cache"], src=a["positions"], dst=a["positions"]), **kw})
+    for call, kw, message in (
+            (append, {"v": a["v"].float()}, "one dtype"), (append, {"q": a["q"]}, "q_out"), (append, {"freqs": a["freqs"].float()}, "freqs"),
+            (append, {"k": a["k"][:, :64]}, "k must be"), (append, {"k": a["k"][:1].expand(4, -1)}, "row stride|HIP device"),
+            (append, {"q": a["q"][:, :100], "q_out": a["q"]}, "heads"), (attend, {"q": a["q"].float()}, "bf16"),
+            (attend, {"slopes": torch.ones(3)}, "slopes"), (attend, {"out": a["out"][:3]}, "out must be"),
+            (rope, {"head_dim": 60}, "heads"), (rope, {"positions": a["positions"].float()}, "int32 or int64"),
+            (rope, {"out": a["out"].float()}, "out is"), (rope, {}, "HIP device"), (copy, {"src": a["positions"][:2]}, "dst"),
+            (copy, {"page_table": a["page_table"]}, "page_map"), (copy, {"k_cache": a["k_cache"][:, :8], "v_cache": a["v_cache"][:, :8]}, "HIP device"),
+            (copy, {"k_cache": a["k_cache"][:, ::2], "v_cache": a["v_cache"][:, ::2]}, "dense"), (copy, {}, "HIP device")):
+        with pytest.raises(abi.HipBackendError, match=message):
+            call(**kw)

@@ -101,6 +101,50 @@ class DecodeDesc(C.Structure):
     ]
 
 
+class RopeDesc(C.Structure):
+    _fields_ = [
+        ("tokens", _i64), ("heads", _i32), ("head_dim", _i32), ("rot_dim", _i32), ("interleaved", _i32),
+        ("inverse", _i32), ("dtype", _i32), ("positions_dtype", _i32), ("scale", C.c_float),
+        ("x", _p), ("ld_x", _i64), ("positions", _p), ("freqs", _p), ("out", _p), ("ld_out", _i64),
+    ]
+
+
+class PagedAppendDesc(C.Structure):
+    _fields_ = [
+        ("tokens", _i64), ("heads_q", _i32), ("heads_kv", _i32), ("head_dim", _i32), ("rot_dim", _i32),
+        ("interleaved", _i32), ("in_dtype", _i32), ("cache_dtype", _i32), ("page_size", _i32),
+        ("n_rows", _i32), ("row_pages", _i32), ("pages", _i64), ("scale", C.c_float), ("pad_", _i32),
+        ("positions", _p), ("rows", _p), ("page_table", _p), ("ld_page_table", _i64), ("freqs", _p),
+        ("q", _p), ("ld_q", _i64), ("q_out", _p), ("ld_q_out", _i64), ("k", _p), ("ld_k", _i64), ("v", _p), ("ld_v", _i64),
+        ("k_cache", _p), ("k_stride_page", _i64), ("k_stride_t", _i64), ("k_stride_h", _i64),
+        ("v_cache", _p), ("v_stride_page", _i64), ("v_stride_t", _i64), ("v_stride_h", _i64),
+        ("k_scale", _p), ("v_scale", _p), ("n_invalid", _p),
+    ]
+
+
+class PagedAttnDesc(C.Structure):
+    _fields_ = [
+        ("tokens", _i32), ("heads_q", _i32), ("heads_kv", _i32), ("head_dim", _i32), ("cache_dtype", _i32),
+        ("page_size", _i32), ("n_rows", _i32), ("row_pages", _i32), ("pages", _i64), ("window", _i32),
+        ("scale", C.c_float), ("softcap", C.c_float), ("pad_", _i32),
+        ("positions", _p), ("rows", _p), ("page_table", _p), ("ld_page_table", _i64), ("q", _p), ("ld_q", _i64),
+        ("k_cache", _p), ("k_stride_page", _i64), ("k_stride_t", _i64), ("k_stride_h", _i64),
+        ("v_cache", _p), ("v_stride_page", _i64), ("v_stride_t", _i64), ("v_stride_h", _i64),
+        ("slopes", _p), ("k_scale", _p), ("v_scale", _p), ("o", _p), ("ld_o", _i64),
+        ("workspace", _p), ("workspace_bytes", _i64),
+    ]
+
+
+class PageCopyDesc(C.Structure):
+    _fields_ = [
+        ("layers", _i32), ("n", _i32), ("pages", _i64), ("page_bytes", _i64),
+        ("k_cache", _p), ("k_layer_bytes", _i64), ("k_page_bytes", _i64),
+        ("v_cache", _p), ("v_layer_bytes", _i64), ("v_page_bytes", _i64),
+        ("src", _p), ("dst", _p), ("page_table", _p), ("ld_page_table", _i64), ("n_rows", _i32), ("row_pages", _i32),
+        ("page_map", _p),
+    ]
+
+
 class SsdDesc(C.Structure):
     _fields_ = [
         ("batch", _i32), ("seq", _i32), ("heads", _i32), ("head_dim", _i32), ("state_dim", _i32), ("ngroups", _i32),
@@ -167,6 +211,11 @@ SIGNATURES: dict[str, tuple] = {
     "th_attention_prefill": (_i32, [C.POINTER(AttnDesc), _p]),
     "th_attention_decode_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32]),
     "th_attention_decode": (_i32, [C.POINTER(DecodeDesc), _p]),
+    "th_rope": (_i32, [C.POINTER(RopeDesc), _p]),
+    "th_paged_append": (_i32, [C.POINTER(PagedAppendDesc), _p]),
+    "th_paged_attention_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32]),
+    "th_paged_attention": (_i32, [C.POINTER(PagedAttnDesc), _p]),
+    "th_page_copy": (_i32, [C.POINTER(PageCopyDesc), _p]),
     "th_epilogue_vm": (_i32, [C.POINTER(VmDesc), _p]),
     "th_ssd_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32]),
     "th_ssd_gtile_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),
