@@ -130,7 +130,7 @@ REFUSED = [
         ({"k_stride_h": 68}, "16 bytes"), ({"v_stride_page": 2050}, "16 bytes"), ({"cache_dtype": 3, "k_stride_t": 136}, "16 bytes"),
         ({"k_stride_t": 1 << 23}, "token strides"), ({"q": 16392}, "16-byte"), ({"v_cache": 65544}, "16-byte"), ({"v_scale": 4096}, "e4m3"),
         ({"tokens": -1}, "tokens"), ({"tokens": 5}, "exceed the table"), ({"positions": 0}, "null"), ({"o": 0}, "null"),
-        ({"row_pages": 1 << 27, "ld_page_table": 1 << 27}, "2^31")]),
+        ({"row_pages": 1 << 27, "ld_page_table": 1 << 27}, "2^30")]),
     ("th_page_copy", copy_desc, [
         ({"layers": 0}, "sizes"), ({"n": -1}, "sizes"), ({"page_bytes": 4104}, "16"), ({"k_cache": 4104}, "16"),
         ({"k_page_bytes": 2048}, "page stride"), ({"v_layer_bytes": 0}, "layer stride"), ({"page_map": 0}, "page table"),
