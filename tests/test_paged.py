@@ -213,12 +213,12 @@ def test_more_argument_checks():
     rope = lambda **kw: ops.rope(**{**dict(x=a["q"], positions=a["positions"], freqs=a["freqs"], out=a["out"], head_dim=64), **kw})
     copy = lambda **kw: ops.copy_pages(**{**dict(k_cache=a["k_cache"], v_cache=a["v_cache"], src=a["positions"], dst=a["positions"]), **kw})
     for call, kw, message in (
-            (append, {"v": a["v"].float()}, "one dtype"), (append, {"q": a["q"]}, "q_out"), (append, {"freqs": a["freqs"].float()}, "freqs"),
+            (append, {"v": a["v"].float()}, "v must be"), (append, {"q": a["q"]}, "q_out"), (append, {"freqs": a["freqs"].float()}, "freqs"),
             (append, {"k": a["k"][:, :64]}, "k must be"), (append, {"k": a["k"][:1].expand(4, -1)}, "row stride|HIP device"),
-            (append, {"q": a["q"][:, :100], "q_out": a["q"]}, "heads"), (attend, {"q": a["q"].float()}, "bf16"),
+            (append, {"q": a["q"][:, :100], "q_out": a["q"]}, "heads"), (attend, {"q": a["q"].float()}, "q must be .* torch.bfloat16"),
             (attend, {"slopes": torch.ones(3)}, "slopes"), (attend, {"out": a["out"][:3]}, "out must be"),
             (rope, {"head_dim": 60}, "heads"), (rope, {"positions": a["positions"].float()}, "int32 or int64"),
-            (rope, {"out": a["out"].float()}, "out is"), (rope, {}, "HIP device"), (copy, {"src": a["positions"][:2]}, "dst"),
+            (rope, {"out": a["out"].float()}, "out must be"), (rope, {}, "HIP device"), (copy, {"src": a["positions"][:2]}, "dst"),
             (copy, {"page_table": a["page_table"]}, "page_map"), (copy, {"k_cache": a["k_cache"][:, :8], "v_cache": a["v_cache"][:, :8]}, "HIP device"),
             (copy, {"k_cache": a["k_cache"][:, ::2], "v_cache": a["v_cache"][:, ::2]}, "dense"), (copy, {}, "HIP device")):
         with pytest.raises(abi.HipBackendError, match=message):

@@ -280,34 +280,49 @@ def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
 
 
 # --------------------------------------------------- rotary positions, paged cache
-def _launch(entry: str, desc: C.Structure, ref: torch.Tensor, kernel: str | None) -> None:
-    """One library call on the device and current stream of ``ref``, whichever device is current."""
-    if ref.device.type == "cuda" and torch.cuda.current_device() != ref.device.index:
-        with torch.cuda.device(ref.device):
-            return _launch(entry, desc, ref, kernel)
-    lib = _lib(ref)
-    abi.check(getattr(lib, entry)(C.byref(desc), _stream(ref)), entry, kernel)
+# One token's calls are shorter on the device than a Python call's bookkeeping, so these take
+# each tensor attribute once, format messages only to raise them and fill a descriptor in one go.
+def _refuse(entry: str, message: str) -> None:
+    raise abi.HipBackendError(entry, abi.TH_ERR_INVALID, message)
 
 
-def _require(ok: bool, entry: str, message: str) -> None:
-    if not ok:
-        raise abi.HipBackendError(entry, abi.TH_ERR_INVALID, message)
+def _launch(entry: str, desc: C.Structure, device: torch.device, kernel: str | None) -> None:
+    """One library call on the current stream of ``device``, whichever device is current."""
+    if device.type != "cuda":
+        _refuse("device", f"tensor on {device}, expected a HIP device")
+    if torch._C._cuda_getDevice() != device.index:
+        with torch.cuda.device(device):
+            return _launch(entry, desc, device, kernel)
+    lib = abi.init_device(device.index)
+    status = getattr(lib, entry)(C.byref(desc), torch._C._cuda_getCurrentRawStream(device.index))
+    if status != abi.TH_OK:
+        abi.check(status, entry, kernel)
 
 
-def _vector(t: torch.Tensor, n: int, dtype: torch.dtype, ref: torch.Tensor, entry: str, name: str) -> int:
-    """Pointer of a contiguous tensor of n values on the device of ``ref``."""
-    _require(t.dtype == dtype and t.numel() == n and t.is_contiguous() and t.device == ref.device, entry,
-             f"{name} must be {n} contiguous {dtype} values on {ref.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+def _vector(t: torch.Tensor, n: int, dtype: torch.dtype, device: torch.device, entry: str, name: str) -> int:
+    """Pointer of n contiguous values on ``device``."""
+    if t.dtype is not dtype or t.numel() != n or not t.is_contiguous() or t.device != device:
+        _refuse(entry, f"{name} must be {n} contiguous {dtype} values on {device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
     return t.data_ptr()
 
 
-def _rows_of(t: torch.Tensor, n: int, width: int, ref: torch.Tensor, entry: str, name: str) -> tuple[int, int]:
-    """(pointer, row stride) of a row-major [n, width] tensor on the device of ``ref``."""
-    _require(t.dim() == 2 and t.shape[0] == n and t.shape[1] == width and (t.stride(1) == 1 or width == 1)
-             and t.device == ref.device, entry,
-             f"{name} must be a row-major [{n}, {width}] tensor on {ref.device}, got {tuple(t.shape)} strides {t.stride()} "
-             f"on {t.device}")
+def _scales(t: torch.Tensor | None, n: int, device: torch.device, entry: str, name: str) -> int | None:
+    return None if t is None else _vector(t, n, torch.float32, device, entry, name)
+
+
+def _rows_of(t: torch.Tensor, n: int, width: int, dtype: torch.dtype, device: torch.device, entry: str, name: str) -> tuple[int, int]:
+    """(pointer, row stride) of a row-major [n, width] tensor on ``device``."""
+    if t.dtype is not dtype or t.shape != (n, width) or (width != 1 and t.stride(1) != 1) or t.device != device:
+        _refuse(entry, f"{name} must be a row-major [{n}, {width}] {dtype} tensor on {device}, got {tuple(t.shape)} strides "
+                       f"{t.stride()} {t.dtype} on {t.device}")
     return t.data_ptr(), t.stride(0) if n > 1 else width
+
+
+def _heads(t: torch.Tensor, head_dim: int, entry: str, name: str) -> tuple[int, int]:
+    """(tokens, width) of a [tokens, heads * head_dim] tensor."""
+    if t.dim() != 2 or head_dim <= 0 or t.shape[1] % head_dim:
+        _refuse(entry, f"{name} {tuple(t.shape)} is no [tokens, heads * {head_dim}] tensor")
+    return t.shape[0], t.shape[1]
 
 
 def rope_frequencies(rot_dim: int, theta: float, *, scaling: str | None = None, factor: float = 1.0,
@@ -322,22 +337,27 @@ def rope_frequencies(rot_dim: int, theta: float, *, scaling: str | None = None, 
     in ``original_len`` positions, divides those that turn less than ``low`` times and blends the
     ones between linearly in their turns (Peng et al. 2023, YaRN; its temperature is
     ``scale = 1 + 0.1 ln(factor)`` of the rotation)."""
-    _require(rot_dim > 0 and rot_dim % 2 == 0, "rope_frequencies", f"rot_dim {rot_dim} must be even and positive")
-    _require(factor > 0.0, "rope_frequencies", f"factor {factor} must be positive")
+    entry = "rope_frequencies"
+    if rot_dim <= 0 or rot_dim % 2:
+        _refuse(entry, f"rot_dim {rot_dim} must be even and positive")
+    if not (factor > 0.0 and theta > 0.0):
+        _refuse(entry, f"theta {theta} and factor {factor} must be positive")
+    if scaling not in (None, "linear", "ntk", "by_parts"):
+        _refuse(entry, f"unknown scaling {scaling!r}")
     i = torch.arange(0, rot_dim, 2, dtype=torch.float64)
     if scaling == "ntk":
-        _require(rot_dim > 2, "rope_frequencies", "ntk scaling needs at least two pairs")
+        if rot_dim == 2:
+            _refuse(entry, "ntk scaling needs at least two pairs")
         theta = theta * factor ** (rot_dim / (rot_dim - 2))
     f = theta ** (-i / rot_dim)
     if scaling == "linear":
         f = f / factor
     elif scaling == "by_parts":
-        _require(original_len > 0 and high > low, "rope_frequencies", "by_parts needs original_len and low < high")
+        if original_len <= 0 or high <= low:
+            _refuse(entry, "by_parts needs original_len and low < high")
         keep = ((f * (original_len / (2 * math.pi)) - low) / (high - low)).clamp(0.0, 1.0)
         f = f * (keep + (1.0 - keep) / factor)
-    else:
-        _require(scaling in (None, "ntk"), "rope_frequencies", f"unknown scaling {scaling!r}")
-    return f.to(device) if device is not None else f
+    return f if device is None else f.to(torch.device("cuda", device) if isinstance(device, int) else device)
 
 
 def rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, out: torch.Tensor, *, head_dim: int,
@@ -347,47 +367,41 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, out: tor
 
     Pairs are dims (i, i + len(freqs)), or (2 i, 2 i + 1) with ``interleaved``; ``scale`` multiplies
     the rotated dims, the others are copied. ``inverse`` turns back: called on the gradient of the
-    output with the same scale it gives the gradient of x. ``out`` may be x."""
-    _require(x.dim() == 2 and head_dim > 0 and x.shape[1] % head_dim == 0, "th_rope",
-             f"x {tuple(x.shape)} is no [tokens, heads * {head_dim}] tensor")
-    _require(positions.dtype in (torch.int32, torch.int64), "th_rope", f"positions are int32 or int64, got {positions.dtype}")
-    _require(out.dtype == x.dtype, "th_rope", f"out is {out.dtype}, x {x.dtype}")
-    n, width = x.shape
-    d = abi.RopeDesc()
-    d.tokens, d.heads, d.head_dim, d.rot_dim = n, width // head_dim, head_dim, 2 * freqs.numel()
-    d.interleaved, d.inverse, d.scale = interleaved, inverse, scale
-    d.dtype, d.positions_dtype = th_dtype(x), th_dtype(positions)
-    d.x, d.ld_x = _rows_of(x, n, width, x, "th_rope", "x")
-    d.out, d.ld_out = _rows_of(out, n, width, x, "th_rope", "out")
-    d.positions = _vector(positions, n, positions.dtype, x, "th_rope", "positions")
-    d.freqs = _vector(freqs, freqs.numel(), torch.float64, x, "th_rope", "freqs")
-    _launch("th_rope", d, x, kernel)
+    output with the same scale it gives the gradient of x. ``out`` may be x; otherwise the two must
+    not overlap."""
+    entry = "th_rope"
+    n, width = _heads(x, head_dim, entry, "x")
+    dev, dt = x.device, x.dtype
+    if positions.dtype not in (torch.int32, torch.int64):
+        _refuse(entry, f"positions are int32 or int64, got {positions.dtype}")
+    half = freqs.numel()
+    xp, ldx = _rows_of(x, n, width, dt, dev, entry, "x")
+    op, ldo = _rows_of(out, n, width, dt, dev, entry, "out")
+    d = abi.RopeDesc(n, width // head_dim, head_dim, 2 * half, interleaved, inverse, th_dtype(dt), _DT[positions.dtype], scale,
+                     xp, ldx, _vector(positions, n, positions.dtype, dev, entry, "positions"),
+                     _vector(freqs, half, torch.float64, dev, entry, "freqs"), op, ldo)
+    _launch(entry, d, dev, kernel)
     return out
 
 
-def _paged_operands(d, entry: str, n: int, ref: torch.Tensor, positions: torch.Tensor, rows: torch.Tensor | None,
-                    k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
-                    k_scale: torch.Tensor | None, v_scale: torch.Tensor | None) -> None:
-    """The fields that the calls on a paged cache share."""
-    _require(k_cache.dim() == 4 and v_cache.shape == k_cache.shape and v_cache.dtype == k_cache.dtype, entry,
-             "k and v caches must be [pages, page_size, heads_kv, head_dim] of one shape and dtype")
-    _require(k_cache.stride(3) == 1 and v_cache.stride(3) == 1, entry, "the head_dim axis of the caches must be contiguous")
-    _require(k_cache.device == ref.device and v_cache.device == ref.device, entry, f"the caches must be on {ref.device}")
-    _require(page_table.dtype == torch.int32 and page_table.dim() == 2, entry, "page_table must be int32 [rows, pages per row]")
-    d.pages, d.page_size, d.heads_kv, d.head_dim = k_cache.shape
-    d.cache_dtype = th_dtype(k_cache)
-    d.n_rows, d.row_pages = page_table.shape
-    d.page_table, d.ld_page_table = _rows_of(page_table, d.n_rows, d.row_pages, ref, entry, "page_table")
-    d.positions = _vector(positions, n, torch.int32, ref, entry, "positions")
-    if rows is not None:
-        d.rows = _vector(rows, n, torch.int32, ref, entry, "rows")
-    d.k_cache, d.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
-    d.k_stride_page, d.k_stride_t, d.k_stride_h, _ = k_cache.stride()
-    d.v_stride_page, d.v_stride_t, d.v_stride_h, _ = v_cache.stride()
-    if k_scale is not None:
-        d.k_scale = _vector(k_scale, d.heads_kv, torch.float32, ref, entry, "k_scale")
-    if v_scale is not None:
-        d.v_scale = _vector(v_scale, d.heads_kv, torch.float32, ref, entry, "v_scale")
+def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, device: torch.device, entry: str) -> tuple:
+    """(shape, strides of k, strides of v) of one layer's caches on ``device``."""
+    shape, ks, vs = k_cache.shape, k_cache.stride(), v_cache.stride()
+    if len(shape) != 4 or v_cache.shape != shape or v_cache.dtype is not k_cache.dtype:
+        _refuse(entry, "k and v caches must be [pages, page_size, heads_kv, head_dim] of one shape and dtype")
+    if ks[3] != 1 or vs[3] != 1:
+        _refuse(entry, "the head_dim axis of the caches must be contiguous")
+    if k_cache.device != device or v_cache.device != device:
+        _refuse(entry, f"the caches must be on {device}")
+    return shape, ks, vs
+
+
+def _table(page_table: torch.Tensor, device: torch.device, entry: str) -> tuple[int, int, int, int]:
+    """(rows, pages per row, pointer, row stride) of a page table on ``device``."""
+    if page_table.dtype is not torch.int32 or page_table.dim() != 2:
+        _refuse(entry, "page_table must be int32 [rows, pages per row]")
+    rows, width = page_table.shape
+    return (rows, width) + _rows_of(page_table, rows, width, torch.int32, device, entry, "page_table")
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -406,32 +420,38 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, k_ca
     outside the table or the cache is left out and counted in ``n_invalid`` (an int32 device
     scalar that the caller zeroes). Two tokens of a call must not share a slot."""
     entry = "th_paged_append"
-    d = abi.PagedAppendDesc()
-    n = k.shape[0]
-    _paged_operands(d, entry, n, k, positions, rows, k_cache, v_cache, page_table, k_scale, v_scale)
-    width = d.heads_kv * d.head_dim
-    _require(v.dtype == k.dtype and (q is None or q.dtype == k.dtype), entry, "q, k and v must share one dtype")
-    d.tokens, d.in_dtype, d.interleaved, d.scale = n, th_dtype(k), interleaved, rope_scale
-    d.k, d.ld_k = _rows_of(k, n, width, k, entry, "k")
-    d.v, d.ld_v = _rows_of(v, n, width, k, entry, "v")
+    n, dev, dt = k.shape[0], k.device, k.dtype
+    (pages, page_size, hk, hd), ks, vs = _cache(k_cache, v_cache, dev, entry)
+    n_rows, row_pages, tp, ldt = _table(page_table, dev, entry)
+    pos = _vector(positions, n, torch.int32, dev, entry, "positions")
+    rp = None if rows is None else _vector(rows, n, torch.int32, dev, entry, "rows")
+    kp, ldk = _rows_of(k, n, hk * hd, dt, dev, entry, "k")
+    vp, ldv = _rows_of(v, n, hk * hd, dt, dev, entry, "v")
+    half, fp = 0, None
     if freqs is not None:
-        d.rot_dim = 2 * freqs.numel()
-        d.freqs = _vector(freqs, freqs.numel(), torch.float64, k, entry, "freqs")
+        half = freqs.numel()
+        fp = _vector(freqs, half, torch.float64, dev, entry, "freqs")
+    hq, qp, ldq, op, ldo = 0, None, 0, None, 0
     if q is not None:
-        _require(q_out is not None and q_out.dtype == torch.bfloat16, entry, "q needs a bf16 q_out")
-        _require(q.dim() == 2 and q.shape[1] % d.head_dim == 0, entry, f"q {tuple(q.shape)} holds no heads of {d.head_dim}")
-        d.heads_q = q.shape[1] // d.head_dim
-        d.q, d.ld_q = _rows_of(q, n, q.shape[1], k, entry, "q")
-        d.q_out, d.ld_q_out = _rows_of(q_out, n, q.shape[1], k, entry, "q_out")
-    if n_invalid is not None:
-        d.n_invalid = _vector(n_invalid, 1, torch.int32, k, entry, "n_invalid")
-    _launch(entry, d, k, kernel)
+        if q_out is None:
+            _refuse(entry, "q needs a q_out")
+        _, width = _heads(q, hd, entry, "q")
+        hq = width // hd
+        qp, ldq = _rows_of(q, n, width, dt, dev, entry, "q")
+        op, ldo = _rows_of(q_out, n, width, torch.bfloat16, dev, entry, "q_out")
+    d = abi.PagedAppendDesc(
+        n, hq, hk, hd, 2 * half, interleaved, th_dtype(dt), th_dtype(k_cache.dtype), page_size, n_rows, row_pages, pages,
+        rope_scale, 0, pos, rp, tp, ldt, fp, qp, ldq, op, ldo, kp, ldk, vp, ldv,
+        k_cache.data_ptr(), ks[0], ks[1], ks[2], v_cache.data_ptr(), vs[0], vs[1], vs[2],
+        _scales(k_scale, hk, dev, entry, "k_scale"), _scales(v_scale, hk, dev, entry, "v_scale"),
+        None if n_invalid is None else _vector(n_invalid, 1, torch.int32, dev, entry, "n_invalid"))
+    _launch(entry, d, dev, kernel)
 
 
 def paged_attention_workspace_bytes(tokens: int, heads_q: int, heads_kv: int, head_dim: int) -> int:
     n = abi.load().th_paged_attention_workspace_bytes(tokens, heads_q, heads_kv, head_dim)
-    _require(n >= 0, "th_paged_attention_workspace_bytes",
-             f"tokens={tokens} heads_q={heads_q} heads_kv={heads_kv} head_dim={head_dim}")
+    if n < 0:
+        _refuse("th_paged_attention_workspace_bytes", f"tokens={tokens} heads_q={heads_q} heads_kv={heads_kv} head_dim={head_dim}")
     return int(n)
 
 
@@ -449,27 +469,28 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``workspace``: :func:`paged_attention_workspace_bytes` bytes that no concurrent call uses;
     without one the call takes it from torch's allocator."""
     entry = "th_paged_attention"
-    d = abi.PagedAttnDesc()
-    n = q.shape[0]
-    _paged_operands(d, entry, n, q, positions, rows, k_cache, v_cache, page_table, k_scale, v_scale)
-    _require(q.dtype == torch.bfloat16 and out.dtype == torch.bfloat16, entry, "q and out must be bf16")
-    _require(q.dim() == 2 and d.head_dim > 0 and q.shape[1] % d.head_dim == 0, entry,
-             f"q {tuple(q.shape)} holds no heads of {d.head_dim}")
-    d.tokens, d.heads_q = n, q.shape[1] // d.head_dim
-    d.scale, d.softcap, d.window = scale, softcap, window
-    d.q, d.ld_q = _rows_of(q, n, q.shape[1], q, entry, "q")
-    d.o, d.ld_o = _rows_of(out, n, q.shape[1], q, entry, "out")
-    if slopes is not None:
-        d.slopes = _vector(slopes, d.heads_q, torch.float32, q, entry, "slopes")
-    if workspace is None and q.device.type == "cuda":
-        abi.init_device(q.device.index)
-        workspace = torch.empty(paged_attention_workspace_bytes(n, d.heads_q, d.heads_kv, d.head_dim), dtype=torch.uint8,
-                                device=q.device)
-    if workspace is not None:
-        _require(workspace.device == q.device and workspace.is_contiguous(), entry,
-                 f"workspace must be a contiguous tensor on {q.device}")
-        d.workspace, d.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    _launch(entry, d, q, kernel)
+    dev = q.device
+    (pages, page_size, hk, hd), ks, vs = _cache(k_cache, v_cache, dev, entry)
+    n, width = _heads(q, hd, entry, "q")
+    n_rows, row_pages, tp, ldt = _table(page_table, dev, entry)
+    pos = _vector(positions, n, torch.int32, dev, entry, "positions")
+    rp = None if rows is None else _vector(rows, n, torch.int32, dev, entry, "rows")
+    hq = width // hd
+    qp, ldq = _rows_of(q, n, width, torch.bfloat16, dev, entry, "q")
+    op, ldo = _rows_of(out, n, width, torch.bfloat16, dev, entry, "out")
+    sp = _scales(slopes, hq, dev, entry, "slopes")
+    if workspace is None:
+        if dev.type == "cuda":
+            abi.init_device(dev.index)
+            workspace = torch.empty(paged_attention_workspace_bytes(n, hq, hk, hd), dtype=torch.uint8, device=dev)
+    elif workspace.device != dev or not workspace.is_contiguous():
+        _refuse(entry, f"workspace must be a contiguous tensor on {dev}")
+    wp, wn = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    d = abi.PagedAttnDesc(
+        n, hq, hk, hd, th_dtype(k_cache.dtype), page_size, n_rows, row_pages, pages, window, scale, softcap, 0, pos, rp, tp, ldt,
+        qp, ldq, k_cache.data_ptr(), ks[0], ks[1], ks[2], v_cache.data_ptr(), vs[0], vs[1], vs[2],
+        sp, _scales(k_scale, hk, dev, entry, "k_scale"), _scales(v_scale, hk, dev, entry, "v_scale"), op, ldo, wp, wn)
+    _launch(entry, d, dev, kernel)
     return out
 
 
@@ -483,35 +504,29 @@ def copy_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, src: torch.Tensor, 
     to ``page_map[p]`` in the same launch: a move. Pairs and entries outside the cache are left
     alone. No page may be both a source and a destination, or twice a destination."""
     entry = "th_page_copy"
-    _require(k_cache.dim() in (4, 5) and v_cache.shape == k_cache.shape and v_cache.dtype == k_cache.dtype
-             and v_cache.device == k_cache.device, entry,
-             "k and v caches must be [layers, pages, page_size, heads_kv, head_dim] of one shape, dtype and device")
-    size = k_cache.element_size()
-    d = abi.PageCopyDesc()
-    d.layers = k_cache.shape[0] if k_cache.dim() == 5 else 1
-    d.pages = k_cache.shape[-4]
-    dense = 1
-    for n in k_cache.shape[-3:]:
-        dense *= n
-    d.page_bytes = dense * size
-    for t, x in ((k_cache, "k"), (v_cache, "v")):
-        run = 1
-        for n, stride in sorted(zip(t.shape[-3:], t.stride()[-3:]), key=lambda a: (a[1], a[0])):
-            _require(n == 1 or stride == run, entry, f"a page of the {x} cache must be one dense block, got strides {t.stride()}")
-            run *= n
-        setattr(d, f"{x}_cache", t.data_ptr())
-        setattr(d, f"{x}_page_bytes", t.stride(-4) * size)
-        setattr(d, f"{x}_layer_bytes", t.stride(0) * size if t.dim() == 5 else 0)
-    d.n = src.numel()
-    d.src = _vector(src, d.n, torch.int32, k_cache, entry, "src")
-    d.dst = _vector(dst, d.n, torch.int32, k_cache, entry, "dst")
+    shape, dev = k_cache.shape, k_cache.device
+    if len(shape) not in (4, 5) or v_cache.shape != shape or v_cache.dtype is not k_cache.dtype or v_cache.device != dev:
+        _refuse(entry, "k and v caches must be [layers, pages, page_size, heads_kv, head_dim] of one shape, dtype and device")
+    size, n = k_cache.element_size(), src.numel()
+    layered, pages = len(shape) == 5, shape[-4]
+    page = shape[-3] * shape[-2] * shape[-1] * size
+    operands = []
+    for t, name in ((k_cache, "k"), (v_cache, "v")):
+        strides, run = t.stride(), 1
+        for stride, extent in sorted(zip(strides[-3:], shape[-3:])):
+            if extent != 1 and stride != run:
+                _refuse(entry, f"a page of the {name} cache must be one dense block, got strides {strides}")
+            run *= extent
+        operands += [t.data_ptr(), strides[0] * size if layered else 0, strides[-4] * size]
+    table = (None, 0, 0, 0, None)
     if page_table is not None:
-        _require(page_map is not None and page_table.dtype == torch.int32 and page_table.dim() == 2, entry,
-                 "renaming takes an int32 [rows, pages per row] page_table and a page_map")
-        d.n_rows, d.row_pages = page_table.shape
-        d.page_table, d.ld_page_table = _rows_of(page_table, d.n_rows, d.row_pages, k_cache, entry, "page_table")
-        d.page_map = _vector(page_map, d.pages, torch.int32, k_cache, entry, "page_map")
-    _launch(entry, d, k_cache, kernel)
+        if page_map is None:
+            _refuse(entry, "renaming a page_table needs a page_map")
+        rows, width, tp, ldt = _table(page_table, dev, entry)
+        table = (tp, ldt, rows, width, _vector(page_map, pages, torch.int32, dev, entry, "page_map"))
+    d = abi.PageCopyDesc(shape[0] if layered else 1, n, pages, page, *operands,
+                         _vector(src, n, torch.int32, dev, entry, "src"), _vector(dst, n, torch.int32, dev, entry, "dst"), *table)
+    _launch(entry, d, dev, kernel)
 
 
 # ----------------------------------------------------------- epilogue VM
