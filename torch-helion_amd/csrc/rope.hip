@@ -13,6 +13,8 @@
 
 #include <math.h>
 
+#include <algorithm>
+
 namespace th {
 
 struct RopeK {
@@ -118,6 +120,203 @@ __global__ void __launch_bounds__(256) rope_elem_kernel(RopeK p) {
   }
 }
 
+// Eight consecutive elements, one 16-byte access for 16-bit types (two for
+// fp32, one of 8 bytes for e4m3).
+template <typename T> struct Pack8;
+template <> struct Pack8<uint16_t> { uint4 w; };
+template <> struct Pack8<float> { float4 w[2]; };
+
+__device__ __forceinline__ void unpack8(const Pack8<uint16_t>& p, float* f) {
+  const uint32_t w[4] = {p.w.x, p.w.y, p.w.z, p.w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(w[i] << 16);
+    f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void unpack8(const Pack8<float>& p, float* f) {
+  *(float4*)f = p.w[0];
+  *(float4*)(f + 4) = p.w[1];
+}
+__device__ __forceinline__ void store8(uint16_t* d, const float* f) {
+  *(uint4*)d = make_uint4(pk_bf16x2(f[0], f[1]), pk_bf16x2(f[2], f[3]), pk_bf16x2(f[4], f[5]), pk_bf16x2(f[6], f[7]));
+}
+__device__ __forceinline__ void store8(float* d, const float* f) {
+  *(float4*)d = *(const float4*)f;
+  *(float4*)(d + 4) = *(const float4*)(f + 4);
+}
+__device__ __forceinline__ void store8(uint8_t* d, const float* f) {
+  int w[2];
+  float c[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c[i] = f[i] != f[i] ? f[i] : fminf(fmaxf(f[i], -448.f), 448.f);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    w[i] = __builtin_amdgcn_cvt_pk_fp8_f32(c[4 * i], c[4 * i + 1], 0, false);
+    w[i] = __builtin_amdgcn_cvt_pk_fp8_f32(c[4 * i + 2], c[4 * i + 3], w[i], true);
+  }
+  *(uint2*)d = make_uint2((unsigned)w[0], (unsigned)w[1]);
+}
+
+constexpr int kMaxTokens = 16;       // tokens of one workgroup
+constexpr int kMaxAngles = 1024;     // their angles
+
+// The usual shapes: rotated halves, heads and strides in whole 16-byte pieces.
+// A thread takes eight pairs at a time (two pieces), or a piece that is only
+// copied, and has the next one's loads under way while it finishes one; the
+// first are issued before the angles are known. tpb tokens share a workgroup,
+// so that a token of few heads does not leave most of it idle.
+template <typename PosT, typename InT, typename OutT, typename CacheT, bool APPEND>
+__global__ void __launch_bounds__(256) rope_vec_kernel(RopeK p, int64_t tokens, int tpb) {
+  __shared__ __attribute__((aligned(16))) float cs[kMaxAngles], sn[kMaxAngles];
+  __shared__ int64_t slot_k[kMaxTokens], slot_v[kMaxTokens];  // -1: not stored
+  __shared__ int live[kMaxTokens];
+  const int64_t t0 = (int64_t)blockIdx.x * tpb;
+  const int nt = (int)min((int64_t)tpb, tokens - t0);
+  const int turns = p.half >> 3, rest = (p.hd - 2 * p.half) >> 3, all = p.hd >> 3;
+  const int heads = p.hq + p.hkv;  // hkv is 0 without APPEND
+  const int n_turn = heads * turns, n_rest = heads * rest;
+  const int units = n_turn + n_rest + p.hkv * all;
+
+  struct Unit {
+    Pack8<InT> a, b;
+    int tok, h, i, kind;  // kind 0: pairs 8 i ..; 1: a copied piece i; 2: piece i of v; -1: none
+  };
+  auto load = [&](int e) {
+    Unit x;
+    x.kind = -1;
+    if (e >= nt * units) return x;
+    x.tok = e / units;
+    e -= x.tok * units;
+    const InT* src;
+    if (e < n_turn) {
+      x.kind = 0;
+      x.h = e / turns;
+      x.i = e - x.h * turns;
+    } else if (e < n_turn + n_rest) {
+      x.kind = 1;
+      e -= n_turn;
+      x.h = e / rest;
+      x.i = e - x.h * rest;
+    } else {
+      x.kind = 2;
+      e -= n_turn + n_rest;
+      x.h = e / all;
+      x.i = e - x.h * all;
+    }
+    const int64_t t = t0 + x.tok;
+    if (x.kind == 2) src = (const InT*)p.v + t * p.ldv + x.h * p.hd;
+    else if (x.h < p.hq) src = (const InT*)p.q + t * p.ldq + x.h * p.hd;
+    else src = (const InT*)p.k + t * p.ldk + (x.h - p.hq) * p.hd;
+    const int at = x.kind == 2 ? 8 * x.i : x.kind == 1 ? 2 * p.half + 8 * x.i : p.interleaved ? 16 * x.i : 8 * x.i;
+    x.a = *(const Pack8<InT>*)(src + at);
+    if (x.kind == 0) x.b = *(const Pack8<InT>*)(src + (p.interleaved ? at + 8 : at + p.half));
+    return x;
+  };
+  Unit cur = load(threadIdx.x);
+
+  for (int e = threadIdx.x; e < nt * p.half; e += 256) {
+    const int tok = e / p.half, i = e - tok * p.half;
+    float s, c;
+    sincospif(2.f * rope_turn(p, ((const PosT*)p.positions)[t0 + tok], i), &s, &c);
+    cs[e] = c * p.scale;
+    sn[e] = s * p.scale * p.sign;
+  }
+  if (APPEND && threadIdx.x < nt) {
+    const int64_t pos = ((const PosT*)p.positions)[t0 + threadIdx.x];
+    int64_t ko = -1, vo = -1;
+    live[threadIdx.x] = pos >= 0;
+    if (pos >= 0 && !cache_slot(p, t0 + threadIdx.x, pos, ko, vo)) {
+      ko = -1;
+      if (p.n_invalid) atomicAdd(p.n_invalid, 1);
+    }
+    slot_k[threadIdx.x] = ko;
+    slot_v[threadIdx.x] = vo;
+  }
+  __syncthreads();
+
+  auto finish = [&](const Unit& x) {
+    if (APPEND && !live[x.tok]) return;
+    const bool query = x.kind != 2 && x.h < p.hq;
+    if (!query && slot_k[x.tok] < 0) return;
+    const int kh = x.kind == 2 ? x.h : x.h - p.hq;
+    float a[8], b[8];
+    unpack8(x.a, a);
+    if (x.kind == 0) {
+      unpack8(x.b, b);
+      const float* c = cs + x.tok * p.half + 8 * x.i;
+      const float* s = sn + x.tok * p.half + 8 * x.i;
+      if (p.interleaved) {  // a: pairs 0..3, b: pairs 4..7
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float u = a[2 * r], v = a[2 * r + 1], w = b[2 * r], z = b[2 * r + 1];
+          a[2 * r] = u * c[r] - v * s[r];
+          a[2 * r + 1] = v * c[r] + u * s[r];
+          b[2 * r] = w * c[4 + r] - z * s[4 + r];
+          b[2 * r + 1] = z * c[4 + r] + w * s[4 + r];
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const float u = a[r], v = b[r];
+          a[r] = u * c[r] - v * s[r];
+          b[r] = v * c[r] + u * s[r];
+        }
+      }
+    }
+    const int at = x.kind == 2 ? 8 * x.i : x.kind == 1 ? 2 * p.half + 8 * x.i : p.interleaved ? 16 * x.i : 8 * x.i;
+    const int bt = p.interleaved ? at + 8 : at + p.half;
+    if (query) {
+      OutT* d = (OutT*)p.qo + (t0 + x.tok) * p.ldqo + x.h * p.hd;
+      store8(d + at, a);
+      if (x.kind == 0) store8(d + bt, b);
+      return;
+    }
+    if constexpr (APPEND) {
+      const float* scales = x.kind == 2 ? p.vs : p.ks;
+      if (scales) {
+        const float m = 1.f / scales[kh];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          a[r] *= m;
+          b[r] *= m;
+        }
+      }
+      CacheT* d = x.kind == 2 ? (CacheT*)p.vc + slot_v[x.tok] + kh * p.vh : (CacheT*)p.kc + slot_k[x.tok] + kh * p.kh;
+      store8(d + at, a);
+      if (x.kind == 0) store8(d + bt, b);
+    }
+  };
+  for (int e = threadIdx.x; e < nt * units; e += 256) {
+    const Unit next = load(e + 256);
+    finish(cur);
+    cur = next;
+  }
+}
+
+static bool whole16(const void* p, int64_t ld, int size) { return ((uintptr_t)p & 15) == 0 && ld * size % 16 == 0; }
+
+template <typename PosT, typename InT, typename OutT, typename CacheT, bool APPEND>
+static void launch_rope(const RopeK& k, int64_t tokens, hipStream_t s) {
+  bool vec = k.half % 8 == 0 && k.half <= kMaxAngles && k.hd % 8 == 0;
+  if (k.hq) vec = vec && whole16(k.q, k.ldq, sizeof(InT)) && whole16(k.qo, k.ldqo, sizeof(OutT));
+  if (APPEND) {
+    // a cache piece is 8 elements: 16 bytes of bf16, 8 of e4m3
+    const uintptr_t mask = 8 * sizeof(CacheT) - 1;
+    vec = vec && whole16(k.k, k.ldk, sizeof(InT)) && whole16(k.v, k.ldv, sizeof(InT)) &&
+          (((uintptr_t)k.kc | (uintptr_t)k.vc) & mask) == 0 && (k.kp | k.kt | k.kh | k.vp | k.vt | k.vh) % 8 == 0;
+  }
+  if (!vec) {
+    hipLaunchKernelGGL((rope_elem_kernel<PosT, InT, OutT, CacheT, APPEND>), dim3((unsigned)tokens), dim3(256), 0, s, k);
+    return;
+  }
+  const int units = (k.hq + k.hkv) * ((k.hd - k.half) >> 3) + k.hkv * (k.hd >> 3);
+  int tpb = std::max(1, std::min(256 / units, kMaxTokens));
+  if (k.half) tpb = std::min(tpb, kMaxAngles / k.half);
+  hipLaunchKernelGGL((rope_vec_kernel<PosT, InT, OutT, CacheT, APPEND>), dim3((unsigned)cdiv(tokens, tpb)), dim3(256), 0, s,
+                     k, tokens, tpb);
+}
+
 }  // namespace th
 
 using namespace th;
@@ -148,15 +347,14 @@ extern "C" int th_rope(const th_rope_desc* d, void* stream) {
   k.positions = d->positions; k.freqs = d->freqs;
   k.scale = d->scale; k.sign = d->inverse ? -1.f : 1.f;
   k.hq = d->heads; k.hd = d->head_dim; k.half = d->rot_dim / 2; k.interleaved = d->interleaved != 0;
-  const dim3 grid((unsigned)d->tokens);
   hipStream_t s = (hipStream_t)stream;
   const bool i64 = d->positions_dtype == TH_I64;
   if (d->dtype == TH_BF16) {
-    if (i64) hipLaunchKernelGGL((rope_elem_kernel<int64_t, uint16_t, uint16_t, uint16_t, false>), grid, dim3(256), 0, s, k);
-    else hipLaunchKernelGGL((rope_elem_kernel<int32_t, uint16_t, uint16_t, uint16_t, false>), grid, dim3(256), 0, s, k);
+    if (i64) launch_rope<int64_t, uint16_t, uint16_t, uint16_t, false>(k, d->tokens, s);
+    else launch_rope<int32_t, uint16_t, uint16_t, uint16_t, false>(k, d->tokens, s);
   } else {
-    if (i64) hipLaunchKernelGGL((rope_elem_kernel<int64_t, float, float, uint16_t, false>), grid, dim3(256), 0, s, k);
-    else hipLaunchKernelGGL((rope_elem_kernel<int32_t, float, float, uint16_t, false>), grid, dim3(256), 0, s, k);
+    if (i64) launch_rope<int64_t, float, float, uint16_t, false>(k, d->tokens, s);
+    else launch_rope<int32_t, float, float, uint16_t, false>(k, d->tokens, s);
   }
   TH_CHECK_LAUNCH();
   return TH_OK;
@@ -209,13 +407,12 @@ extern "C" int th_paged_append(const th_paged_append_desc* d, void* stream) {
   k.kc = d->k_cache; k.kp = d->k_stride_page; k.kt = d->k_stride_t; k.kh = d->k_stride_h;
   k.vc = d->v_cache; k.vp = d->v_stride_page; k.vt = d->v_stride_t; k.vh = d->v_stride_h;
   k.ks = d->k_scale; k.vs = d->v_scale; k.n_invalid = d->n_invalid;
-  const dim3 grid((unsigned)d->tokens);
   hipStream_t s = (hipStream_t)stream;
   const bool f32 = d->in_dtype == TH_F32, e4 = d->cache_dtype == TH_F8E4M3;
-  if (f32 && e4) hipLaunchKernelGGL((rope_elem_kernel<int32_t, float, uint16_t, uint8_t, true>), grid, dim3(256), 0, s, k);
-  else if (f32) hipLaunchKernelGGL((rope_elem_kernel<int32_t, float, uint16_t, uint16_t, true>), grid, dim3(256), 0, s, k);
-  else if (e4) hipLaunchKernelGGL((rope_elem_kernel<int32_t, uint16_t, uint16_t, uint8_t, true>), grid, dim3(256), 0, s, k);
-  else hipLaunchKernelGGL((rope_elem_kernel<int32_t, uint16_t, uint16_t, uint16_t, true>), grid, dim3(256), 0, s, k);
+  if (f32 && e4) launch_rope<int32_t, float, uint16_t, uint8_t, true>(k, d->tokens, s);
+  else if (f32) launch_rope<int32_t, float, uint16_t, uint16_t, true>(k, d->tokens, s);
+  else if (e4) launch_rope<int32_t, uint16_t, uint16_t, uint8_t, true>(k, d->tokens, s);
+  else launch_rope<int32_t, uint16_t, uint16_t, uint16_t, true>(k, d->tokens, s);
   TH_CHECK_LAUNCH();
   return TH_OK;
 }
