@@ -50,6 +50,7 @@ struct PAttnK {
   int n_rows, row_pages, pshift;
   int tokens, Hkv, G, nqb, gq;  // nqb blocks of gq <= 16 query heads per kv head
   int window;
+  int o8;           // o in whole 8-byte pieces
   float scale, softcap;
   const float* slopes;
   const float* ks;
@@ -71,19 +72,24 @@ __device__ __forceinline__ void pa_lds_order() {
 }
 
 // A token's keys: [lo, hi) of its row; tiles start at lo rounded down to 16.
-struct Span { int lo, hi, base, tiles; };
+struct Span { int pos, row, lo, hi, base, tiles; };
 
 template <int KT>
-__device__ __forceinline__ Span span_of(const PAttnK& p, int t) {
+__device__ __forceinline__ Span span_from(const PAttnK& p, int pos, int row) {
   Span s;
-  const int64_t pos = p.positions[t];
-  const int row = p.rows ? p.rows[t] : t;
+  s.pos = pos;
+  s.row = row;
   const bool in = row >= 0 && row < p.n_rows && pos >= 0;
-  s.hi = in ? (int)min(pos + 1, (int64_t)p.row_pages << p.pshift) : 0;
-  s.lo = p.window ? (int)max((int64_t)0, pos + 1 - p.window) : 0;
+  s.hi = in ? (int)min((int64_t)pos + 1, (int64_t)p.row_pages << p.pshift) : 0;
+  s.lo = p.window ? (int)max((int64_t)0, (int64_t)pos + 1 - p.window) : 0;
   s.base = s.lo & ~15;
   s.tiles = s.hi > s.lo ? (s.hi - s.base + KT - 1) / KT : 0;
   return s;
+}
+
+template <int KT>
+__device__ __forceinline__ Span span_of(const PAttnK& p, int t) {
+  return span_from<KT>(p, p.positions[t], p.rows ? p.rows[t] : t);
 }
 
 // Equal stretches of n tiles over w waves: the first n % w get one more.
@@ -191,7 +197,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PAttnK p) {
     sp = span_of<KT>(p, ++t);
   }
   int64_t u = u0;
-  int hb, k0;  // kv head block; first tile of it
+  int hb, k;  // kv head block; tile of it
   {
     const int64_t rel = u0 - at * HB;
     if (rel >> 31) {
@@ -199,8 +205,11 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PAttnK p) {
     } else {
       hb = (int)((uint32_t)rel / (uint32_t)sp.tiles);
     }
-    k0 = (int)(rel - (int64_t)hb * sp.tiles);
+    k = (int)(rel - (int64_t)hb * sp.tiles);
   }
+  t = __builtin_amdgcn_readfirstlane(t);
+  hb = __builtin_amdgcn_readfirstlane(hb);
+  k = __builtin_amdgcn_readfirstlane(k);
 
   char* sv = smem + wave * T::LDS;
   // V: lane's row and chunk within one load instruction
@@ -212,196 +221,239 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PAttnK p) {
   const int vxo = pa_sw<D>(vr0) >> 1;
   const char* rv = sv + vr0 * D * 2 + (j4 >> 1) * 16 + (j4 & 1) * 8;
 
-  while (u < u1) {
-    // ---- one segment: tiles k0 .. k1 of pair (t, hb)
-    t = __builtin_amdgcn_readfirstlane(t);
-    hb = __builtin_amdgcn_readfirstlane(hb);
-    k0 = __builtin_amdgcn_readfirstlane(k0);
-    const int kvh = hb / p.nqb, qb = hb - kvh * p.nqb;
-    const int k1 = (int)min((int64_t)sp.tiles, k0 + (u1 - u));
-    const int lo = sp.lo, hi = sp.hi, base = sp.base;
-    const int row = p.rows ? p.rows[t] : t;
-    const int32_t* trow = p.table + (int64_t)row * p.ldt;
-    const int h0 = kvh * p.G + qb * 16;                 // first query head
-    const int gn = min(p.gq, p.G - qb * 16);            // query heads here
+  // ---- the load cursor (t, hb, k; sp): one tile ahead of the computation, also
+  // over the ends of pairs and tokens
+  // (the next token's position and row wait in vector registers: a scalar copy
+  // would make the compiler wait for them where they are loaded)
+  const int last_t = p.tokens - 1;
+  int vzero = 0;
+  asm volatile("" : "+v"(vzero));
+  int npos, nrow = 0;
+  auto load_next = [&]() {
+    const int at_ = min(t + 1, last_t) + vzero;
+    npos = p.positions[at_];
+    if (p.rows) nrow = p.rows[at_];
+  };
+  load_next();
+  // page numbers p0 .. p0 + 63 of the row, one a lane (-1: not in the cache)
+  int p0 = 1 << 30, ids = -1;
+  unsigned okbits = 0;  // bit b: block b of the loaded tile is in the cache
+  pa_u32x4 kr[8], vr[8];
+  auto load = [&]() {
+    const int kvh = hb / p.nqb;
     const char* kb = p.k + (int64_t)kvh * p.kh;
     const char* vb = p.v + (int64_t)kvh * p.vh;
-
-    bf16x8_t qf[NKS];
-    const uint16_t* qrow = p.q + (int64_t)t * p.ldq + (int64_t)(h0 + qc) * D;
-#pragma unroll
-    for (int ks = 0; ks < NKS; ++ks) {
-      const int dim = E4 ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1) : 32 * ks + 8 * g;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) qf[ks][e] = (__bf16)0.f;
-      if (qc < gn) qf[ks] = *(const bf16x8_t*)(qrow + dim);
+    const int j0 = sp.base + k * KT;
+    const int first = j0 >> p.pshift, last = (min(j0 + KT, sp.hi) - 1) >> p.pshift;
+    if (first < p0 || last - p0 >= 64) {
+      p0 = first;
+      const int at_ = p0 + lane;
+      ids = at_ < p.row_pages ? p.table[(int64_t)sp.row * p.ldt + at_] : -1;
+      if (ids >= p.pages) ids = -1;
     }
-    float mul = p.scale * (p.ks ? p.ks[kvh] : 1.f);
-    // capped: softcap log2(e) tanh(mul s / softcap), else mul log2(e) s
-    const bool cap = p.softcap > 0.f;
-    mul *= cap ? 2.f * kLog2e / p.softcap : kLog2e;
-    const float capl = p.softcap * kLog2e;
-    const float slope = p.slopes && qc < gn ? p.slopes[h0 + qc] * kLog2e : 0.f;
-    const int pos = p.positions[t];
-
-    // page numbers p0 .. p0 + 63 of the row, one a lane (-1: not in the cache)
-    int p0 = -64, ids = -1;
-    unsigned okbits = 0;  // bit b: block b of the loaded tile is in the cache
-    pa_u32x4 kr[8], vr[8];
-    auto load = [&](int k) {
-      const int j0 = base + k * KT;
-      const int first = j0 >> p.pshift, last = (min(j0 + KT, hi) - 1) >> p.pshift;
-      if (last - p0 >= 64) {
-        p0 = first;
-        const int at_ = p0 + lane;
-        ids = at_ < p.row_pages ? trow[at_] : -1;
-        if (ids >= p.pages) ids = -1;
-      }
-      okbits = 0;
+    okbits = 0;
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const int jb = j0 + 16 * b;
-        const int id = __builtin_amdgcn_readlane(ids, ((jb >> p.pshift) - p0) & 63);
-        const int in = jb & ((1 << p.pshift) - 1);
-        const int rows = min(16, hi - jb);          // rows of this block below hi
-        const bool ok = id >= 0 && rows > 0;
-        okbits |= (ok ? 1u : 0u) << b;
-        const char* kpage = kb + (int64_t)(ok ? id : 0) * p.kp + (int64_t)in * p.kt;
-        const char* vpage = vb + (int64_t)(ok ? id : 0) * p.vp + (int64_t)in * p.vt;
-        const auto kres = __builtin_amdgcn_make_buffer_rsrc((void*)kpage, 0, ok ? (int)((rows - 1) * p.kt) + RB : 0, 0x00020000);
-        const auto vres = __builtin_amdgcn_make_buffer_rsrc((void*)vpage, 0, ok ? (int)((rows - 1) * p.vt) + RB : 0, 0x00020000);
+    for (int b = 0; b < NB; ++b) {
+      const int jb = j0 + 16 * b;
+      const int id = __builtin_amdgcn_readlane(ids, ((jb >> p.pshift) - p0) & 63);
+      const int in = jb & ((1 << p.pshift) - 1);
+      const int rows = min(16, sp.hi - jb);       // rows of this block below hi
+      const bool ok = id >= 0 && rows > 0;
+      okbits |= (ok ? 1u : 0u) << b;
+      const char* kpage = kb + (int64_t)(ok ? id : 0) * p.kp + (int64_t)in * p.kt;
+      const char* vpage = vb + (int64_t)(ok ? id : 0) * p.vp + (int64_t)in * p.vt;
+      const auto kres = __builtin_amdgcn_make_buffer_rsrc((void*)kpage, 0, ok ? (int)((rows - 1) * p.kt) + RB : 0, 0x00020000);
+      const auto vres = __builtin_amdgcn_make_buffer_rsrc((void*)vpage, 0, ok ? (int)((rows - 1) * p.vt) + RB : 0, 0x00020000);
 #pragma unroll
-        for (int j = 0; j < JPR; ++j)
-          kr[b * JPR + j] = __builtin_bit_cast(
-              pa_u32x4, __builtin_amdgcn_raw_buffer_load_b128(kres, qc * (int)p.kt + 64 * j + 16 * g, 0, 0));
+      for (int j = 0; j < JPR; ++j)
+        kr[b * JPR + j] = __builtin_bit_cast(
+            pa_u32x4, __builtin_amdgcn_raw_buffer_load_b128(kres, qc * (int)p.kt + 64 * j + 16 * g, 0, 0));
 #pragma unroll
-        for (int i = 0; i < 16 / RPI; ++i) {
-          const int r = i * RPI + lr;
-          const int off = jb + r >= lo ? r * (int)p.vt + 16 * lc : 0x7ffffff0;
-          vr[b * (16 / RPI) + i] = __builtin_bit_cast(pa_u32x4, __builtin_amdgcn_raw_buffer_load_b128(vres, off, 0, 0));
-        }
-      }
-    };
-
-    f32x4_t oacc[NDB];
-#pragma unroll
-    for (int d = 0; d < NDB; ++d)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) oacc[d][r] = 0.f;
-    float m_run = -INFINITY, l_run = 0.f;
-
-    load(k0);
-    for (int k = k0; k < k1; ++k) {
-      const int j0 = base + k * KT;
-      const unsigned ok = okbits;
-      pa_lds_order();
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 16 / RPI; ++i) {
         const int r = i * RPI + lr;
-        if constexpr (E4) {
-          char* w = sv + r * D * 2 + (((2 * lc) ^ pa_sw<D>(r)) << 4);
-          *(bf16x8_t*)w = e4m3x8_to_bf16(vr[i][0], vr[i][1]);
-          *(bf16x8_t*)(w + 16) = e4m3x8_to_bf16(vr[i][2], vr[i][3]);
-        } else {
-          *(pa_u32x4*)(sv + r * D * 2 + ((lc ^ pa_sw<D>(r)) << 4)) = vr[i];
-        }
+        const int off = jb + r >= sp.lo ? r * (int)p.vt + 16 * lc : 0x7ffffff0;
+        vr[b * (16 / RPI) + i] = __builtin_bit_cast(pa_u32x4, __builtin_amdgcn_raw_buffer_load_b128(vres, off, 0, 0));
       }
-      f32x4_t s[NB];
+    }
+  };
+  // the pair's queries and scalars; a column past its heads repeats the last one
+  // (no lane depends on another's column, and none of them is stored)
+  bf16x8_t qn[NKS];
+  float kscale_n = 1.f, slope_n = 0.f;
+  auto load_pair = [&]() {
+    const int kvh = hb / p.nqb, qb = hb - kvh * p.nqb;
+    const int head = kvh * p.G + qb * 16 + min(qc, min(p.gq, p.G - qb * 16) - 1);
+    const uint16_t* qrow = p.q + (int64_t)t * p.ldq + (int64_t)head * D;
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[b][r] = 0.f;
-#pragma unroll
-        for (int j = 0; j < JPR; ++j) {
-          const pa_u32x4 x = kr[b * JPR + j];
-          if constexpr (E4) {
-            s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e4m3x8_to_bf16(x[0], x[1]), qf[2 * j], s[b], 0, 0, 0);
-            s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e4m3x8_to_bf16(x[2], x[3]), qf[2 * j + 1], s[b], 0, 0, 0);
-          } else {
-            s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x), qf[j], s[b], 0, 0, 0);
-          }
-        }
-      }
-      if (k + 1 < k1) load(k + 1);
-      pa_lds_order();
+    for (int ks = 0; ks < NKS; ++ks)
+      qn[ks] = *(const bf16x8_t*)(qrow + (E4 ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1) : 32 * ks + 8 * g));
+    if (p.ks) kscale_n = p.ks[kvh];
+    if (p.slopes) slope_n = p.slopes[head];
+  };
 
-      // scores in log2 units; this lane holds keys 16 b + 4 g + r of column qc
+  bf16x8_t qf[NKS];
+  f32x4_t oacc[NDB];
+  float m_run = 0.f, l_run = 0.f, mul = 0.f, slope = 0.f;
+  // capped: softcap log2(e) tanh(mul s / (2 log2(e))), else mul s
+  const bool cap = p.softcap > 0.f;
+  const float mul0 = p.scale * (cap ? 2.f * kLog2e / p.softcap : kLog2e);
+  const float capl = p.softcap * kLog2e;
+  int k_begin = 0;
+  int64_t u_begin = u0;
+  bool fresh = true;
+  load();
+  load_pair();
+  for (;;) {
+    // ---- one tile of pair (ct, chb)
+    const int ct = t, chb = hb, ck = k;
+    const Span cs = sp;
+    const unsigned ok = okbits;
+    const int j0 = cs.base + ck * KT;
+    if (fresh) {
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float x = s[b][r] * mul;
-          if (cap) x = capl - 2.f * capl * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x));
-          s[b][r] = x;
-        }
-      if (p.slopes) {
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s[b][r] -= slope * (float)(pos - (j0 + 16 * b + 4 * g + r));
-      }
-      if (j0 < lo || j0 + KT > hi || ok != (1u << NB) - 1) {
-#pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int j = j0 + 16 * b + 4 * g + r;
-            if (j < lo || j >= hi || !(ok >> b & 1)) s[b][r] = -INFINITY;
-          }
-      }
-      float mloc = -INFINITY;
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) mloc = fmaxf(mloc, s[b][r]);
-      mloc = fmaxf(mloc, __shfl_xor(mloc, 16));
-      mloc = fmaxf(mloc, __shfl_xor(mloc, 32));
-      const float m_new = fmaxf(m_run, mloc);
-      const float m_use = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
-      m_run = m_new;
-      float lsum = 0.f;
-      bf16x8_t pf[NB / 2];
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float e = __builtin_amdgcn_exp2f(s[b][r] - m_use);
-          lsum += e;
-          pf[b / 2][4 * (b & 1) + r] = (__bf16)e;
-        }
-      l_run = l_run * alpha + lsum;
+      for (int ks = 0; ks < NKS; ++ks) qf[ks] = qn[ks];
 #pragma unroll
       for (int d = 0; d < NDB; ++d)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) oacc[d][r] *= alpha;
+        for (int r = 0; r < 4; ++r) oacc[d][r] = 0.f;
+      m_run = -INFINITY;
+      l_run = 0.f;
+      mul = mul0 * kscale_n;
+      slope = slope_n * kLog2e;
+      k_begin = ck;
+      u_begin = u;
+    }
+    pa_lds_order();
 #pragma unroll
-      for (int b = 0; b < NB / 2; ++b)
+    for (int i = 0; i < 8; ++i) {
+      const int r = i * RPI + lr;
+      if constexpr (E4) {
+        char* w = sv + r * D * 2 + (((2 * lc) ^ pa_sw<D>(r)) << 4);
+        *(bf16x8_t*)w = e4m3x8_to_bf16(vr[i][0], vr[i][1]);
+        *(bf16x8_t*)(w + 16) = e4m3x8_to_bf16(vr[i][2], vr[i][3]);
+      } else {
+        *(pa_u32x4*)(sv + r * D * 2 + ((lc ^ pa_sw<D>(r)) << 4)) = vr[i];
+      }
+    }
+    f32x4_t s[NB];
 #pragma unroll
-        for (int db = 0; db < NDB; ++db) {
-          const char* x = rv + b * 32 * D * 2 + ((db ^ vxo) << 5);
-          const pa_s16x4 vlo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pa_s16x4*)x);
-          const pa_s16x4 vhi =
-              __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pa_s16x4*)(x + 16 * D * 2));
-          const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(vlo, vhi, 0, 1, 2, 3, 4, 5, 6, 7));
-          oacc[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[b], oacc[db], 0, 0, 0);
+    for (int b = 0; b < NB; ++b) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s[b][r] = 0.f;
+#pragma unroll
+      for (int j = 0; j < JPR; ++j) {
+        const pa_u32x4 x = kr[b * JPR + j];
+        if constexpr (E4) {
+          s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e4m3x8_to_bf16(x[0], x[1]), qf[2 * j], s[b], 0, 0, 0);
+          s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e4m3x8_to_bf16(x[2], x[3]), qf[2 * j + 1], s[b], 0, 0, 0);
+        } else {
+          s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x), qf[j], s[b], 0, 0, 0);
+        }
+      }
+    }
+    ++u;
+    const bool more = u < u1, ends = !more || ck + 1 == cs.tiles;
+    if (more) {
+      if (++k == sp.tiles) {
+        k = 0;
+        if (++hb == HB) {
+          hb = 0;
+          ++t;
+          sp = span_from<KT>(p, __builtin_amdgcn_readfirstlane(npos), p.rows ? __builtin_amdgcn_readfirstlane(nrow) : t);
+          while (sp.tiles == 0) sp = span_of<KT>(p, ++t);
+          load_next();
+          p0 = 1 << 30;
+        }
+      }
+      load();
+      if (ends) load_pair();
+    }
+    pa_lds_order();
+
+    // scores in log2 units; this lane holds keys 16 b + 4 g + r of column qc
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float x = s[b][r] * mul;
+        if (cap) x = capl - 2.f * capl * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x));
+        s[b][r] = x;
+      }
+    if (p.slopes) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[b][r] -= slope * (float)(cs.pos - (j0 + 16 * b + 4 * g + r));
+    }
+    if (j0 < cs.lo || j0 + KT > cs.hi || ok != (1u << NB) - 1) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int j = j0 + 16 * b + 4 * g + r;
+          if (j < cs.lo || j >= cs.hi || !(ok >> b & 1)) s[b][r] = -INFINITY;
         }
     }
+    float mloc = -INFINITY;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) mloc = fmaxf(mloc, s[b][r]);
+    mloc = fmaxf(mloc, __shfl_xor(mloc, 16));
+    mloc = fmaxf(mloc, __shfl_xor(mloc, 32));
+    const float m_new = fmaxf(m_run, mloc);
+    const float m_use = m_new == -INFINITY ? 0.f : m_new;
+    const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
+    m_run = m_new;
+    float lsum = 0.f;
+    bf16x8_t pf[NB / 2];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float e = __builtin_amdgcn_exp2f(s[b][r] - m_use);
+        lsum += e;
+        pf[b / 2][4 * (b & 1) + r] = (__bf16)e;
+      }
+    l_run = l_run * alpha + lsum;
+#pragma unroll
+    for (int d = 0; d < NDB; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) oacc[d][r] *= alpha;
+#pragma unroll
+    for (int b = 0; b < NB / 2; ++b)
+#pragma unroll
+      for (int db = 0; db < NDB; ++db) {
+        const char* x = rv + b * 32 * D * 2 + ((db ^ vxo) << 5);
+        const pa_s16x4 vlo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pa_s16x4*)x);
+        const pa_s16x4 vhi =
+            __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pa_s16x4*)(x + 16 * D * 2));
+        const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(vlo, vhi, 0, 1, 2, 3, 4, 5, 6, 7));
+        oacc[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[b], oacc[db], 0, 0, 0);
+      }
+    fresh = ends;
+    if (!ends) continue;
 
-    // ---- the segment's result: the output, or a part for the join
+    // ---- the pair's result here: the output, or a part for the join
     float l = l_run + __shfl_xor(l_run, 16);
     l += __shfl_xor(l, 32);
-    if (qc < gn) {
-      if (k0 == 0 && k1 == sp.tiles) {
+    const int kvh = chb / p.nqb, qb = chb - kvh * p.nqb;
+    if (qc < min(p.gq, p.G - qb * 16)) {
+      if (k_begin == 0 && ck + 1 == cs.tiles) {
         const float f = l == 0.f ? 0.f : (p.vs ? p.vs[kvh] : 1.f) / l;
-        uint16_t* o = p.o + (int64_t)t * p.ldo + (int64_t)(h0 + qc) * D + 4 * g;
+        uint16_t* o = p.o + (int64_t)ct * p.ldo + (int64_t)(kvh * p.G + qb * 16 + qc) * D + 4 * g;
 #pragma unroll
         for (int db = 0; db < NDB; ++db) {
+          if (p.o8) {
+            *(uint2*)(o + 16 * db) = make_uint2(pk_bf16x2(oacc[db][0] * f, oacc[db][1] * f),
+                                                pk_bf16x2(oacc[db][2] * f, oacc[db][3] * f));
+          } else {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) o[16 * db + r] = f32_to_bf16(oacc[db][r] * f);
+            for (int r = 0; r < 4; ++r) o[16 * db + r] = f32_to_bf16(oacc[db][r] * f);
+          }
         }
       } else {
-        const int64_t slot = (int64_t)(2 * me + (u != u0)) * p.gq + qc;
+        const int64_t slot = (int64_t)(2 * me + (u_begin != u0)) * p.gq + qc;
         if (g == 0) {
           p.ml[2 * slot] = m_run;
           p.ml[2 * slot + 1] = l;
@@ -410,13 +462,7 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PAttnK p) {
         for (int db = 0; db < NDB; ++db) *(f32x4_t*)(p.part + slot * D + 16 * db + 4 * g) = oacc[db];
       }
     }
-    u += k1 - k0;
-    k0 = 0;
-    if (u < u1 && ++hb == HB) {
-      hb = 0;
-      do sp = span_of<KT>(p, ++t);
-      while (sp.tiles == 0);
-    }
+    if (!more) break;
   }
 }
 
@@ -545,6 +591,7 @@ extern "C" int th_paged_attention(const th_paged_attn_desc* d, void* stream) {
   k.n_rows = d->n_rows; k.row_pages = d->row_pages; k.pshift = __builtin_ctz((unsigned)d->page_size);
   k.tokens = d->tokens; k.Hkv = d->heads_kv; k.G = d->heads_q / d->heads_kv;
   k.gq = std::min(k.G, 16); k.nqb = (int)cdiv(k.G, 16);
+  k.o8 = d->ld_o % 4 == 0 && ((uintptr_t)d->o & 7) == 0;
   k.window = d->window; k.scale = d->scale; k.softcap = d->softcap;
   k.slopes = d->slopes; k.ks = d->k_scale; k.vs = d->v_scale;
   const int grid = paged_grid();
