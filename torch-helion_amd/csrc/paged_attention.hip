@@ -8,13 +8,21 @@
 // enough of them are in flight, and that all CUs have the same amount to read.
 //
 // Work: a tile is 8 KiB of K and 8 KiB of V (KT keys of one kv head), whatever
-// the head size and type. The tiles of all (token, kv head) pairs form one
-// line, and each of the 4 * grid waves takes an equal stretch of it, so ragged
-// batches, one long sequence and many short ones are dealt out alike, with
-// nothing about the lengths known on the host (a captured graph serves any
-// lengths). A wave walks its stretch alone, with no workgroup barrier. The
-// parts of a pair that was cut go through the workspace (m, l, o in fp32) to
-// the join kernel; a pair inside one stretch is finished by its wave.
+// the head size and type. Two forms deal the tiles out:
+//   line     the key tiles of all tokens form one line; the waves (eight a CU)
+//            form groups with one wave for each kv head, and each group takes an
+//            equal stretch of the line, so ragged batches, one long sequence and
+//            many short ones are dealt out alike, with nothing about the lengths
+//            known on the host (a captured graph serves any lengths). The parts
+//            of a token that was cut go through the workspace (m, l, o in fp32)
+//            to the join kernel; a token inside one stretch is finished by its
+//            group. The waves of a CU keep step with a barrier a tile: left
+//            alone, the older half of them is served first and ends at 108 us
+//            where the younger ends at 134 (64 sequences of 2048-4096 keys); and
+//            the heads of a key, neighbours in memory, are read together.
+//   pair     a workgroup of four waves for each pair, its tiles dealt out in turn
+//            and the waves merged in LDS: where a pair can have only a few tiles
+//            by its table and window, one launch and no line to lay out.
 //
 // One tile:
 //   K        loaded straight in the operand layout of S^T = K Q^T
@@ -55,9 +63,9 @@ struct PAttnK {
   const float* slopes;
   const float* ks;
   const float* vs;
-  int64_t* prefix;  // [tokens + 1]: tiles of one kv head of the tokens before
-  float* ml;        // [2 waves][gq][2]
-  float* part;      // [2 waves][gq][D], unnormalised
+  int64_t* prefix;  // line: [tokens + 1], tiles of the tokens before
+  float* ml;        // line: [2 waves][gq][2]
+  float* part;      // line: [2 waves][gq][D], unnormalised
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -71,10 +79,10 @@ __device__ __forceinline__ void pa_lds_order() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// A token's keys: [lo, hi) of its row; tiles start at lo rounded down to 16.
-struct Span { int pos, row, lo, hi, base, tiles; };
+// A token's keys: [lo, hi) of its row; units start at lo rounded down to 16.
+struct Span { int pos, row, lo, hi, base, units; };  // units of KU keys
 
-template <int KT>
+template <int KU>
 __device__ __forceinline__ Span span_from(const PAttnK& p, int pos, int row) {
   Span s;
   s.pos = pos;
@@ -83,16 +91,16 @@ __device__ __forceinline__ Span span_from(const PAttnK& p, int pos, int row) {
   s.hi = in ? (int)min((int64_t)pos + 1, (int64_t)p.row_pages << p.pshift) : 0;
   s.lo = p.window ? (int)max((int64_t)0, (int64_t)pos + 1 - p.window) : 0;
   s.base = s.lo & ~15;
-  s.tiles = s.hi > s.lo ? (s.hi - s.base + KT - 1) / KT : 0;
+  s.units = s.hi > s.lo ? (s.hi - s.base + KU - 1) / KU : 0;
   return s;
 }
 
-template <int KT>
+template <int KU>
 __device__ __forceinline__ Span span_of(const PAttnK& p, int t) {
-  return span_from<KT>(p, p.positions[t], p.rows ? p.rows[t] : t);
+  return span_from<KU>(p, p.positions[t], p.rows ? p.rows[t] : t);
 }
 
-// Equal stretches of n tiles over w waves: the first n % w get one more.
+// Equal stretches of n tiles over w groups: the first n % w get one more.
 struct Share {
   int64_t each, more;
   __device__ __forceinline__ Share(int64_t n, int w) {
@@ -139,25 +147,47 @@ struct PaTile {
   static constexpr int LDS = KT * D * 2;        // one wave's V tile, bf16
 };
 
-template <int D, bool E4>
-__global__ void __launch_bounds__(256, 2) paged_attn_kernel(PAttnK p) {
+constexpr int kLineWaves = 8, kPairWaves = 4;  // waves of a workgroup
+
+template <int D, bool E4, bool PAIR>
+__global__ void __launch_bounds__(64 * (PAIR ? kPairWaves : kLineWaves), PAIR ? 2 : 1) paged_attn_kernel(PAttnK p) {
   using T = PaTile<D, E4>;
+  constexpr int NW = PAIR ? kPairWaves : kLineWaves;
+  constexpr int KU = PAIR ? NW * T::KT : T::KT;  // keys of a step: of the workgroup's, or of one wave's
   constexpr int RB = T::RB, KT = T::KT, NB = T::NB, CPR = T::CPR, RPI = T::RPI;
   constexpr int NKS = D / 32, NDB = D / 16, JPR = RB / 64;  // JPR: K loads per 16-key block
-  __shared__ __attribute__((aligned(16))) char smem[4 * T::LDS];
-  __shared__ int64_t pre[257];
-  __shared__ int64_t wsum[4];
+  constexpr int OW = PAIR ? NW * 16 * D * 4 : 0;  // the merge's o rows share the V tiles' LDS
+  __shared__ __attribute__((aligned(16))) char smem[NW * T::LDS > OW ? NW * T::LDS : OW];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int qc = lane & 15, g = lane >> 4;  // query column, lane group
-
-  // ---- tiles before each of 256 runs of tokens
-  const int per = (p.tokens + 255) >> 8;
-  {
+  const int HB = p.Hkv * p.nqb;
+  int me;          // pair: the pair; line: the wave's number, group by group
+  int64_t u0, u1;  // the stretch; where it begins:
+  int t, hb, k;    // token, kv head block, unit of the token
+  int64_t steps = 0, step = 0;  // line: the barriers that the waves keep step with
+  Span sp;
+  if constexpr (PAIR) {
+    me = blockIdx.x;
+    t = me / HB;
+    hb = me - t * HB;
+    k = 0;
+    sp = span_of<KU>(p, t);
+    u0 = 0;
+    u1 = sp.units;
+    if (u1 == 0) {
+      const int kvh = hb / p.nqb, qb = hb - kvh * p.nqb, gn = min(p.gq, p.G - qb * 16);
+      for (int e = tid; e < gn * D; e += 64 * NW) p.o[(int64_t)t * p.ldo + (int64_t)(kvh * p.G + qb * 16) * D + e] = 0;
+      return;
+    }
+  } else {
+    __shared__ int64_t pre[64 * NW + 1];  // tiles before each of 64 NW runs of tokens
+    __shared__ int64_t wsum[NW];
+    const int per = (p.tokens + 64 * NW - 1) / (64 * NW);
     int64_t n = 0;
-    const int t0 = tid * per, t1 = min(p.tokens, t0 + per);
-    for (int t = t0; t < t1; ++t) n += span_of<KT>(p, t).tiles;
+    const int t0 = min(p.tokens, tid * per), t1 = min(p.tokens, t0 + per);
+    for (int i = t0; i < t1; ++i) n += span_of<KU>(p, i).units;
     int64_t inc = n;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -169,44 +199,42 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PAttnK p) {
     int64_t before = inc - n;
     for (int w = 0; w < wave; ++w) before += wsum[w];
     pre[tid] = before;
-    if (tid == 255) pre[256] = before + n;
+    if (tid == 64 * NW - 1) pre[64 * NW] = before + n;
     if (blockIdx.x == 0) {  // for the join kernel
       int64_t at = before;
-      for (int t = t0; t < t1; ++t) {
-        p.prefix[t] = at;
-        at += span_of<KT>(p, t).tiles;
+      for (int i = t0; i < t1; ++i) {
+        p.prefix[i] = at;
+        at += span_of<KU>(p, i).units;
       }
-      if (tid == 255) p.prefix[p.tokens] = before + n;
+      if (tid == 64 * NW - 1) p.prefix[p.tokens] = before + n;
     }
     __syncthreads();
-  }
-  const int HB = p.Hkv * p.nqb;
-  const Share share(pre[256] * HB, gridDim.x * 4);
-  const int me = wave * gridDim.x + blockIdx.x;  // few tiles: one wave per workgroup first
-  const int64_t u0 = share.begin(me), u1 = share.begin(me + 1);
-  if (u0 >= u1) return;
-
-  // ---- the pair and tile that the stretch begins in
-  int t = 0;
-  for (int i = 0; i < 4; ++i) t += __popcll(__ballot(pre[64 * i + lane] * HB <= u0));
-  t = (t - 1) * per;  // the last run that begins at or before u0
-  int64_t at = pre[t / per];
-  Span sp = span_of<KT>(p, t);
-  while ((at + sp.tiles) * HB <= u0) {
-    at += sp.tiles;
-    sp = span_of<KT>(p, ++t);
+    const int groups = (int)gridDim.x * NW / HB;
+    const Share share(pre[64 * NW], groups);
+    if (share.each) steps = share.each + (share.more != 0);
+    // no step to keep (a tile a wave at most): neighbours on different CUs, so
+    // that few tiles spread out
+    me = steps ? (int)blockIdx.x * NW + wave : wave * (int)gridDim.x + (int)blockIdx.x;
+    const int group = me / HB;
+    hb = me - group * HB;
+    u0 = share.begin(group);
+    u1 = group < groups ? share.begin(group + 1) : u0;
+    if (u0 >= u1) {
+      for (; step < steps; ++step) barrier_keep_loads();
+      return;
+    }
+    int run = -1;  // the last run that begins at or before u0
+    for (int i = 0; i < NW; ++i) run += __popcll(__ballot(pre[64 * i + lane] <= u0));
+    t = run * per;
+    int64_t at = pre[run];
+    sp = span_of<KU>(p, t);
+    while (at + sp.units <= u0) {
+      at += sp.units;
+      sp = span_of<KU>(p, ++t);
+    }
+    k = (int)(u0 - at);
   }
   int64_t u = u0;
-  int hb, k;  // kv head block; tile of it
-  {
-    const int64_t rel = u0 - at * HB;
-    if (rel >> 31) {
-      hb = (int)(rel / sp.tiles);
-    } else {
-      hb = (int)((uint32_t)rel / (uint32_t)sp.tiles);
-    }
-    k = (int)(rel - (int64_t)hb * sp.tiles);
-  }
   t = __builtin_amdgcn_readfirstlane(t);
   hb = __builtin_amdgcn_readfirstlane(hb);
   k = __builtin_amdgcn_readfirstlane(k);
@@ -221,8 +249,8 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PAttnK p) {
   const int vxo = pa_sw<D>(vr0) >> 1;
   const char* rv = sv + vr0 * D * 2 + (j4 >> 1) * 16 + (j4 & 1) * 8;
 
-  // ---- the load cursor (t, hb, k; sp): one tile ahead of the computation, also
-  // over the ends of pairs and tokens
+  // ---- the load cursor (t, k; sp): one tile ahead of the computation, also over the
+  // ends of tokens
   // (the next token's position and row wait in vector registers: a scalar copy
   // would make the compiler wait for them where they are loaded)
   const int last_t = p.tokens - 1;
@@ -243,7 +271,9 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PAttnK p) {
     const int kvh = hb / p.nqb;
     const char* kb = p.k + (int64_t)kvh * p.kh;
     const char* vb = p.v + (int64_t)kvh * p.vh;
-    const int j0 = sp.base + k * KT;
+    const int j0 = sp.base + (PAIR ? NW * k + wave : k) * KT;
+    okbits = 0;
+    if (j0 >= sp.hi) return;  // past the pair's end: this wave sits the unit out
     const int first = j0 >> p.pshift, last = (min(j0 + KT, sp.hi) - 1) >> p.pshift;
     if (first < p0 || last - p0 >= 64) {
       p0 = first;
@@ -251,7 +281,6 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PAttnK p) {
       ids = at_ < p.row_pages ? p.table[(int64_t)sp.row * p.ldt + at_] : -1;
       if (ids >= p.pages) ids = -1;
     }
-    okbits = 0;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       const int jb = j0 + 16 * b;
@@ -304,11 +333,12 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PAttnK p) {
   load();
   load_pair();
   for (;;) {
-    // ---- one tile of pair (ct, chb)
-    const int ct = t, chb = hb, ck = k;
+    // ---- one unit of pair (ct, hb)
+    const int ct = t, ck = k;
     const Span cs = sp;
     const unsigned ok = okbits;
-    const int j0 = cs.base + ck * KT;
+    const int j0 = cs.base + (PAIR ? NW * ck + wave : ck) * KT;
+    const bool busy = j0 < cs.hi;
     if (fresh) {
 #pragma unroll
       for (int ks = 0; ks < NKS; ++ks) qf[ks] = qn[ks];
@@ -323,135 +353,172 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PAttnK p) {
       k_begin = ck;
       u_begin = u;
     }
-    pa_lds_order();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = i * RPI + lr;
-      if constexpr (E4) {
-        char* w = sv + r * D * 2 + (((2 * lc) ^ pa_sw<D>(r)) << 4);
-        *(bf16x8_t*)w = e4m3x8_to_bf16(vr[i][0], vr[i][1]);
-        *(bf16x8_t*)(w + 16) = e4m3x8_to_bf16(vr[i][2], vr[i][3]);
-      } else {
-        *(pa_u32x4*)(sv + r * D * 2 + ((lc ^ pa_sw<D>(r)) << 4)) = vr[i];
-      }
-    }
     f32x4_t s[NB];
+    if (busy) {
+      pa_lds_order();
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) s[b][r] = 0.f;
-#pragma unroll
-      for (int j = 0; j < JPR; ++j) {
-        const pa_u32x4 x = kr[b * JPR + j];
+      for (int i = 0; i < 8; ++i) {
+        const int r = i * RPI + lr;
         if constexpr (E4) {
-          s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e4m3x8_to_bf16(x[0], x[1]), qf[2 * j], s[b], 0, 0, 0);
-          s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e4m3x8_to_bf16(x[2], x[3]), qf[2 * j + 1], s[b], 0, 0, 0);
+          char* w = sv + r * D * 2 + (((2 * lc) ^ pa_sw<D>(r)) << 4);
+          *(bf16x8_t*)w = e4m3x8_to_bf16(vr[i][0], vr[i][1]);
+          *(bf16x8_t*)(w + 16) = e4m3x8_to_bf16(vr[i][2], vr[i][3]);
         } else {
-          s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x), qf[j], s[b], 0, 0, 0);
+          *(pa_u32x4*)(sv + r * D * 2 + ((lc ^ pa_sw<D>(r)) << 4)) = vr[i];
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[b][r] = 0.f;
+#pragma unroll
+        for (int j = 0; j < JPR; ++j) {
+          const pa_u32x4 x = kr[b * JPR + j];
+          if constexpr (E4) {
+            s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e4m3x8_to_bf16(x[0], x[1]), qf[2 * j], s[b], 0, 0, 0);
+            s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e4m3x8_to_bf16(x[2], x[3]), qf[2 * j + 1], s[b], 0, 0, 0);
+          } else {
+            s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x), qf[j], s[b], 0, 0, 0);
+          }
         }
       }
     }
     ++u;
-    const bool more = u < u1, ends = !more || ck + 1 == cs.tiles;
+    const bool more = u < u1, ends = !more || ck + 1 == cs.units;
     if (more) {
-      if (++k == sp.tiles) {
+      if (++k == sp.units) {
         k = 0;
-        if (++hb == HB) {
-          hb = 0;
-          ++t;
-          sp = span_from<KT>(p, __builtin_amdgcn_readfirstlane(npos), p.rows ? __builtin_amdgcn_readfirstlane(nrow) : t);
-          while (sp.tiles == 0) sp = span_of<KT>(p, ++t);
-          load_next();
-          p0 = 1 << 30;
-        }
+        ++t;
+        sp = span_from<KU>(p, __builtin_amdgcn_readfirstlane(npos), p.rows ? __builtin_amdgcn_readfirstlane(nrow) : t);
+        while (sp.units == 0) sp = span_of<KU>(p, ++t);
+        load_next();
+        p0 = 1 << 30;
       }
       load();
       if (ends) load_pair();
     }
-    pa_lds_order();
+    if (busy) {
+      pa_lds_order();
 
-    // scores in log2 units; this lane holds keys 16 b + 4 g + r of column qc
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float x = s[b][r] * mul;
-        if (cap) x = capl - 2.f * capl * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x));
-        s[b][r] = x;
-      }
-    if (p.slopes) {
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s[b][r] -= slope * (float)(cs.pos - (j0 + 16 * b + 4 * g + r));
-    }
-    if (j0 < cs.lo || j0 + KT > cs.hi || ok != (1u << NB) - 1) {
+      // scores in log2 units; this lane holds keys 16 b + 4 g + r of column qc
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int j = j0 + 16 * b + 4 * g + r;
-          if (j < cs.lo || j >= cs.hi || !(ok >> b & 1)) s[b][r] = -INFINITY;
+          float x = s[b][r] * mul;
+          if (cap) x = capl - 2.f * capl * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x));
+          s[b][r] = x;
+        }
+      if (p.slopes) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[b][r] -= slope * (float)(cs.pos - (j0 + 16 * b + 4 * g + r));
+      }
+      if (j0 < cs.lo || j0 + KT > cs.hi || ok != (1u << NB) - 1) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int j = j0 + 16 * b + 4 * g + r;
+            if (j < cs.lo || j >= cs.hi || !(ok >> b & 1)) s[b][r] = -INFINITY;
+          }
+      }
+      float mloc = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) mloc = fmaxf(mloc, s[b][r]);
+      mloc = fmaxf(mloc, __shfl_xor(mloc, 16));
+      mloc = fmaxf(mloc, __shfl_xor(mloc, 32));
+      const float m_new = fmaxf(m_run, mloc);
+      const float m_use = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
+      m_run = m_new;
+      float lsum = 0.f;
+      bf16x8_t pf[NB / 2];
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float e = __builtin_amdgcn_exp2f(s[b][r] - m_use);
+          lsum += e;
+          pf[b / 2][4 * (b & 1) + r] = (__bf16)e;
+        }
+      l_run = l_run * alpha + lsum;
+#pragma unroll
+      for (int d = 0; d < NDB; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) oacc[d][r] *= alpha;
+#pragma unroll
+      for (int b = 0; b < NB / 2; ++b)
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) {
+          const char* x = rv + b * 32 * D * 2 + ((db ^ vxo) << 5);
+          const pa_s16x4 vlo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pa_s16x4*)x);
+          const pa_s16x4 vhi =
+              __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pa_s16x4*)(x + 16 * D * 2));
+          const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(vlo, vhi, 0, 1, 2, 3, 4, 5, 6, 7));
+          oacc[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[b], oacc[db], 0, 0, 0);
         }
     }
-    float mloc = -INFINITY;
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) mloc = fmaxf(mloc, s[b][r]);
-    mloc = fmaxf(mloc, __shfl_xor(mloc, 16));
-    mloc = fmaxf(mloc, __shfl_xor(mloc, 32));
-    const float m_new = fmaxf(m_run, mloc);
-    const float m_use = m_new == -INFINITY ? 0.f : m_new;
-    const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
-    m_run = m_new;
-    float lsum = 0.f;
-    bf16x8_t pf[NB / 2];
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float e = __builtin_amdgcn_exp2f(s[b][r] - m_use);
-        lsum += e;
-        pf[b / 2][4 * (b & 1) + r] = (__bf16)e;
-      }
-    l_run = l_run * alpha + lsum;
-#pragma unroll
-    for (int d = 0; d < NDB; ++d)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) oacc[d][r] *= alpha;
-#pragma unroll
-    for (int b = 0; b < NB / 2; ++b)
-#pragma unroll
-      for (int db = 0; db < NDB; ++db) {
-        const char* x = rv + b * 32 * D * 2 + ((db ^ vxo) << 5);
-        const pa_s16x4 vlo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pa_s16x4*)x);
-        const pa_s16x4 vhi =
-            __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pa_s16x4*)(x + 16 * D * 2));
-        const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(vlo, vhi, 0, 1, 2, 3, 4, 5, 6, 7));
-        oacc[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[b], oacc[db], 0, 0, 0);
-      }
+    if (step < steps) {
+      barrier_keep_loads();
+      ++step;
+    }
     fresh = ends;
     if (!ends) continue;
 
     // ---- the pair's result here: the output, or a part for the join
     float l = l_run + __shfl_xor(l_run, 16);
     l += __shfl_xor(l, 32);
-    const int kvh = chb / p.nqb, qb = chb - kvh * p.nqb;
-    if (qc < min(p.gq, p.G - qb * 16)) {
-      if (k_begin == 0 && ck + 1 == cs.tiles) {
-        const float f = l == 0.f ? 0.f : (p.vs ? p.vs[kvh] : 1.f) / l;
-        uint16_t* o = p.o + (int64_t)ct * p.ldo + (int64_t)(kvh * p.G + qb * 16 + qc) * D + 4 * g;
+    const int kvh = hb / p.nqb, qb = hb - kvh * p.nqb;
+    const int gn = min(p.gq, p.G - qb * 16);
+    const float vscale = p.vs ? p.vs[kvh] : 1.f;
+    uint16_t* o = p.o + (int64_t)ct * p.ldo + (int64_t)(kvh * p.G + qb * 16) * D;
+    auto put4 = [&](uint16_t* at, const f32x4_t x, float f) {
+      if (p.o8) {
+        *(uint2*)at = make_uint2(pk_bf16x2(x[0] * f, x[1] * f), pk_bf16x2(x[2] * f, x[3] * f));
+      } else {
 #pragma unroll
-        for (int db = 0; db < NDB; ++db) {
-          if (p.o8) {
-            *(uint2*)(o + 16 * db) = make_uint2(pk_bf16x2(oacc[db][0] * f, oacc[db][1] * f),
-                                                pk_bf16x2(oacc[db][2] * f, oacc[db][3] * f));
-          } else {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[16 * db + r] = f32_to_bf16(oacc[db][r] * f);
-          }
+        for (int r = 0; r < 4; ++r) at[r] = f32_to_bf16(x[r] * f);
+      }
+    };
+    if constexpr (PAIR) {  // one pair, one result: the waves are merged
+      __shared__ float mw[NW][16], lw[NW][16];
+      float(*ow)[16][D] = (float(*)[16][D])smem;
+      lds_barrier();  // every wave is done with its V tile
+      if (qc < gn) {
+        if (g == 0) {
+          mw[wave][qc] = m_run;
+          lw[wave][qc] = l;
         }
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) *(f32x4_t*)&ow[wave][qc][16 * db + 4 * g] = oacc[db];
+      }
+      lds_barrier();
+      for (int e = tid; e < gn * (D / 4); e += 64 * NW) {
+        const int c = e / (D / 4), d4 = e % (D / 4) * 4;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) mx = fmaxf(mx, mw[w][c]);
+        const float mu = mx == -INFINITY ? 0.f : mx;
+        float lt = 0.f;
+        f32x4_t x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          const float f = __builtin_amdgcn_exp2f(mw[w][c] - mu);
+          const f32x4_t y = *(const f32x4_t*)&ow[w][c][d4];
+          lt += lw[w][c] * f;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[r] += y[r] * f;
+        }
+        put4(o + c * D + d4, x, lt == 0.f ? 0.f : vscale / lt);
+      }
+    } else if (qc < gn) {
+      if (k_begin == 0 && ck + 1 == cs.units) {
+#pragma unroll
+        for (int db = 0; db < NDB; ++db) put4(o + qc * D + 16 * db + 4 * g, oacc[db], l == 0.f ? 0.f : vscale / l);
       } else {
         const int64_t slot = (int64_t)(2 * me + (u_begin != u0)) * p.gq + qc;
         if (g == 0) {
@@ -464,69 +531,66 @@ __global__ void __launch_bounds__(256, 2) paged_attn_kernel(PAttnK p) {
     }
     if (!more) break;
   }
+  for (; step < steps; ++step) barrier_keep_loads();
 }
 
-// Joins the parts of one (token, query head): o = sum_i o_i 2^(m_i - m) / sum_i
-// l_i 2^(m_i - m). Tokens without keys get zeros; pairs that one wave finished
-// are left alone.
+// Joins the parts of hw heads of one (token, kv head) pair: o = sum_i o_i
+// 2^(m_i - m) / sum_i l_i 2^(m_i - m). Tokens without keys get zeros; pairs that
+// one wave finished are left alone.
 template <int D>
-__global__ void __launch_bounds__(256) paged_attn_join_kernel(PAttnK p, int waves) {
+__global__ void __launch_bounds__(256) paged_attn_join_kernel(PAttnK p, int waves, int hw) {
   constexpr int LPR = D / 4, NG = 256 / LPR;  // lanes per row, rows at a time
-  __shared__ float red[4];
-  __shared__ float ls[NG];
   __shared__ f32x4_t os[NG][LPR];
-  const int h = blockIdx.x, t = blockIdx.y, tid = threadIdx.x;
-  const int kvh = h / p.G, in = h - kvh * p.G, qb = in >> 4, qc = in & 15;
-  const int HB = p.Hkv * p.nqb, hb = kvh * p.nqb + qb;
-  const int64_t a = p.prefix[t], tiles = p.prefix[t + 1] - a;
-  uint16_t* o = p.o + (int64_t)t * p.ldo + (int64_t)h * D;
+  __shared__ float ms[NG], ls[NG];
+  const int HB = p.Hkv * p.nqb, per = (p.gq + hw - 1) / hw;  // workgroups per pair
+  const int hb = blockIdx.x / per, c0 = (blockIdx.x - hb * per) * hw, t = blockIdx.y, tid = threadIdx.x;
+  const int kvh = hb / p.nqb, qb = hb - kvh * p.nqb, gn = min(p.gq, p.G - qb * 16);
+  const int64_t a = p.prefix[t], tiles = p.prefix[t + 1] - a, all = p.prefix[p.tokens];
+  uint16_t* o = p.o + (int64_t)t * p.ldo + (int64_t)(kvh * p.G + qb * 16) * D;
   if (tiles == 0) {
-    if (tid < D) o[tid] = 0;
+    for (int e = c0 * D + tid; e < min(gn, c0 + hw) * D; e += 256) o[e] = 0;
     return;
   }
-  const Share share(p.prefix[p.tokens] * HB, waves);
-  const int64_t b0 = a * HB + hb * tiles;
-  const int w0 = share.owner(b0), n = share.owner(b0 + tiles - 1) - w0 + 1;
+  const Share share(all, waves / HB);
+  const int g0 = share.owner(a), n = share.owner(a + tiles - 1) - g0 + 1;
   if (n == 1) return;
-  // part i is wave w0 + i's: its first segment's, or its last where that is another
-  auto slot_of = [&](int i) {
-    const int w = w0 + i;
-    return (int64_t)(2 * w + (i == 0 && b0 != share.begin(w))) * p.gq + qc;
-  };
-  float mx = -INFINITY;
-  for (int i = tid; i < n; i += 256) mx = fmaxf(mx, p.ml[2 * slot_of(i)]);
-#pragma unroll
-  for (int x = 32; x; x >>= 1) mx = fmaxf(mx, __shfl_xor(mx, x));
-  if ((tid & 63) == 0) red[tid >> 6] = mx;
-  __syncthreads();
-  mx = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const float mu = mx == -INFINITY ? 0.f : mx;
+  const bool late = a != share.begin(g0);  // part 0 is its wave's last segment, not its first
+  const float vscale = p.vs ? p.vs[kvh] : 1.f;
+  // rows at a time: hw heads, and as many slices of the parts as that leaves
   const int grp = tid / LPR, ln = tid - grp * LPR;
-  float l = 0.f;
-  f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int i = grp; i < n; i += NG) {
-    const int64_t s = slot_of(i);
-    const float f = __builtin_amdgcn_exp2f(p.ml[2 * s] - mu);
-    l += p.ml[2 * s + 1] * f;
-    const f32x4_t x = *(const f32x4_t*)(p.part + s * D + 4 * ln);
+  const int slices = NG / hw, slice = grp / hw, c = c0 + grp - slice * hw;
+  float m = -INFINITY, l = 0.f;
+  f32x4_t x = {0.f, 0.f, 0.f, 0.f};
+  auto add = [&](float mi, float li, const f32x4_t y) {
+    const float mn = fmaxf(m, mi), mu = mn == -INFINITY ? 0.f : mn;
+    const float fo = __builtin_amdgcn_exp2f(m - mu), fi = __builtin_amdgcn_exp2f(mi - mu);
+    m = mn;
+    l = l * fo + li * fi;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) acc[r] += x[r] * f;
+    for (int r = 0; r < 4; ++r) x[r] = x[r] * fo + y[r] * fi;
+  };
+  if (c < gn && slice < slices) {
+#pragma unroll 8
+    for (int i = slice; i < n; i += slices) {
+      const int64_t s = (int64_t)(2 * ((g0 + i) * HB + hb) + (i == 0 && late)) * p.gq + c;
+      add(p.ml[2 * s], p.ml[2 * s + 1], *(const f32x4_t*)(p.part + s * D + 4 * ln));
+    }
   }
-  os[grp][ln] = acc;
-  if (ln == 0) ls[grp] = l;
+  os[grp][ln] = x;
+  if (ln == 0) {
+    ms[grp] = m;
+    ls[grp] = l;
+  }
   __syncthreads();
-  if (tid >= D) return;
-  float ll = 0.f, oo = 0.f;
+  if (slice != 0 || c >= gn) return;
+  for (int i = 1; i < slices; ++i) add(ms[i * hw + grp], ls[i * hw + grp], os[i * hw + grp][ln]);
+  const float f = l == 0.f ? 0.f : vscale / l;
 #pragma unroll
-  for (int i = 0; i < NG; ++i) {
-    ll += ls[i];
-    oo += os[i][tid >> 2][tid & 3];
-  }
-  o[tid] = f32_to_bf16(ll == 0.f ? 0.f : oo / ll * (p.vs ? p.vs[kvh] : 1.f));
+  for (int r = 0; r < 4; ++r) o[c * D + 4 * ln + r] = f32_to_bf16(x[r] * f);
 }
 
-static int paged_grid() { return 2 * (device_cus() > 0 ? device_cus() : 256); }
+// One workgroup of eight waves per CU.
+static int line_grid() { return device_cus() > 0 ? device_cus() : 256; }
 
 }  // namespace th
 
@@ -534,7 +598,7 @@ using namespace th;
 
 extern "C" int64_t th_paged_attention_workspace_bytes(int32_t tokens, int32_t heads_q, int32_t heads_kv, int32_t head_dim) {
   if (tokens < 0 || heads_q <= 0 || heads_kv <= 0 || heads_q % heads_kv || (head_dim != 64 && head_dim != 128)) return -1;
-  const int64_t gq = std::min(heads_q / heads_kv, 16), slots = (int64_t)paged_grid() * 4 * 2;
+  const int64_t gq = std::min(heads_q / heads_kv, 16), slots = (int64_t)line_grid() * kLineWaves * 2;
   return cdiv((int64_t)(tokens + 1) * 8, 16) * 16 + cdiv(slots * gq * 2 * 4, 16) * 16 + slots * gq * head_dim * 4;
 }
 
@@ -569,6 +633,8 @@ extern "C" int th_paged_attention(const th_paged_attn_desc* d, void* stream) {
   TH_CHECK_ARG((!d->k_scale && !d->v_scale) || d->cache_dtype == TH_F8E4M3,
                "th_paged_attention: scales need an e4m3 cache");
   if (d->tokens == 0) return TH_OK;
+  TH_CHECK_ARG(d->heads_kv * cdiv(d->heads_q / d->heads_kv, 16) <= 256,
+               "th_paged_attention: more than 256 kv heads (each 16 query heads of one count)");
   TH_CHECK_ARG(d->rows || d->tokens <= d->n_rows, "th_paged_attention: %d tokens without rows exceed the table's %d",
                d->tokens, d->n_rows);
   TH_CHECK_ARG(d->q && d->k_cache && d->v_cache && d->o && d->positions && d->page_table,
@@ -594,26 +660,45 @@ extern "C" int th_paged_attention(const th_paged_attn_desc* d, void* stream) {
   k.o8 = d->ld_o % 4 == 0 && ((uintptr_t)d->o & 7) == 0;
   k.window = d->window; k.scale = d->scale; k.softcap = d->softcap;
   k.slopes = d->slopes; k.ks = d->k_scale; k.vs = d->v_scale;
-  const int grid = paged_grid();
+  const int grid = line_grid(), waves = grid * kLineWaves;
   char* ws = (char*)d->workspace;
   k.prefix = (int64_t*)ws;
   ws += cdiv((int64_t)(d->tokens + 1) * 8, 16) * 16;
   k.ml = (float*)ws;
-  ws += cdiv((int64_t)grid * 8 * k.gq * 8, 16) * 16;
+  ws += cdiv((int64_t)waves * 2 * k.gq * 8, 16) * 16;
   k.part = (float*)ws;
   hipStream_t s = (hipStream_t)stream;
   const bool e4 = d->cache_dtype == TH_F8E4M3;
+  // The most tiles that a pair can have, by its table and window: up to 16 of them
+  // (four for each wave) take the pair form.
+  const int64_t keys = std::min<int64_t>((int64_t)d->row_pages * d->page_size, d->window ? (int64_t)d->window + 15 : INT64_MAX);
+  const int64_t pairs = (int64_t)d->tokens * d->heads_kv * k.nqb;
+  if (cdiv(keys * d->head_dim * es, 8192) <= 16 && pairs < (int64_t)1 << 31) {
+    const dim3 g((unsigned)pairs), b(64 * kPairWaves);
+    if (d->head_dim == 128) {
+      if (e4) hipLaunchKernelGGL((paged_attn_kernel<128, true, true>), g, b, 0, s, k);
+      else hipLaunchKernelGGL((paged_attn_kernel<128, false, true>), g, b, 0, s, k);
+    } else {
+      if (e4) hipLaunchKernelGGL((paged_attn_kernel<64, true, true>), g, b, 0, s, k);
+      else hipLaunchKernelGGL((paged_attn_kernel<64, false, true>), g, b, 0, s, k);
+    }
+    TH_CHECK_LAUNCH();
+    return TH_OK;
+  }
+  const dim3 g(grid), b(64 * kLineWaves);
   if (d->head_dim == 128) {
-    if (e4) hipLaunchKernelGGL((paged_attn_kernel<128, true>), dim3(grid), dim3(256), 0, s, k);
-    else hipLaunchKernelGGL((paged_attn_kernel<128, false>), dim3(grid), dim3(256), 0, s, k);
+    if (e4) hipLaunchKernelGGL((paged_attn_kernel<128, true, false>), g, b, 0, s, k);
+    else hipLaunchKernelGGL((paged_attn_kernel<128, false, false>), g, b, 0, s, k);
   } else {
-    if (e4) hipLaunchKernelGGL((paged_attn_kernel<64, true>), dim3(grid), dim3(256), 0, s, k);
-    else hipLaunchKernelGGL((paged_attn_kernel<64, false>), dim3(grid), dim3(256), 0, s, k);
+    if (e4) hipLaunchKernelGGL((paged_attn_kernel<64, true, false>), g, b, 0, s, k);
+    else hipLaunchKernelGGL((paged_attn_kernel<64, false, false>), g, b, 0, s, k);
   }
   TH_CHECK_LAUNCH();
-  const dim3 jgrid(d->heads_q, d->tokens);
-  if (d->head_dim == 128) hipLaunchKernelGGL(paged_attn_join_kernel<128>, jgrid, dim3(256), 0, s, k, 4 * grid);
-  else hipLaunchKernelGGL(paged_attn_join_kernel<64>, jgrid, dim3(256), 0, s, k, 4 * grid);
+  // few pairs: a workgroup for each head, so that their many parts are read at once
+  const int hw = pairs >= 256 ? std::min(k.gq, 1024 / d->head_dim) : 1;
+  const dim3 join((unsigned)(d->heads_kv * k.nqb * cdiv(k.gq, hw)), (unsigned)d->tokens);
+  if (d->head_dim == 128) hipLaunchKernelGGL(paged_attn_join_kernel<128>, join, dim3(256), 0, s, k, waves, hw);
+  else hipLaunchKernelGGL(paged_attn_join_kernel<64>, join, dim3(256), 0, s, k, waves, hw);
   TH_CHECK_LAUNCH();
   return TH_OK;
 }
