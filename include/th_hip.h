@@ -367,7 +367,7 @@ int th_paged_append(const th_paged_append_desc* desc, void* stream);
  * key (padded, or of a row outside the table) gets zeros. What the slots of
  * unseen keys hold, NaN included, does not reach the result. The keys of all
  * tokens are dealt out evenly over the GPU, whatever the lengths, and the
- * parts are joined through the workspace.
+ * parts are joined through the workspace (which short rows do not need).
  */
 typedef struct th_paged_attn_desc {
   int32_t tokens, heads_q, heads_kv, head_dim;  /* head_dim 64 or 128 */
@@ -391,8 +391,11 @@ typedef struct th_paged_attn_desc {
   float* workspace; int64_t workspace_bytes;  /* 16-byte aligned; holds nothing between calls */
 } th_paged_attn_desc;
 
-/* Workspace th_paged_attention needs for these sizes on the current device (-1: bad sizes). */
-int64_t th_paged_attention_workspace_bytes(int32_t tokens, int32_t heads_q, int32_t heads_kv, int32_t head_dim);
+/* Workspace th_paged_attention needs for these sizes on the current device, with
+ * max_keys = row_pages * page_size (0: none, rows so short that nothing is
+ * joined; -1: bad sizes). */
+int64_t th_paged_attention_workspace_bytes(int32_t tokens, int32_t heads_q, int32_t heads_kv, int32_t head_dim,
+                                           int32_t cache_dtype, int64_t max_keys, int32_t window);
 
 int th_paged_attention(const th_paged_attn_desc* desc, void* stream);
 

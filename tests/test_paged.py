@@ -170,9 +170,21 @@ def test_null_empty_and_valid_descriptors(lib, entry, make, empty):
 
 
 def test_workspace_query(lib):
-    for bad in ((-1, 8, 2, 64), (4, 0, 2, 64), (4, 8, 3, 64), (4, 8, 2, 96), (4, 8, 0, 64)):
-        assert lib.th_paged_attention_workspace_bytes(*bad) == -1
-    assert lib.th_paged_attention_workspace_bytes(4, 8, 2, 64) >= 0
+    from torch_helion.hip import abi, ops
+
+    good = dict(tokens=4, heads_q=8, heads_kv=2, head_dim=64, cache_dtype=abi.TH_BF16, max_keys=4096, window=0)
+    query = lambda **kw: lib.th_paged_attention_workspace_bytes(*{**good, **kw}.values())
+    for bad in ({"tokens": -1}, {"heads_q": 0}, {"heads_kv": 3}, {"head_dim": 96}, {"heads_kv": 0}, {"cache_dtype": abi.TH_F32},
+                {"max_keys": 0}, {"window": -1}, {"max_keys": 1 << 30}):
+        assert query(**bad) == -1, bad
+    assert query() > 0 and query(tokens=0) == 0
+    # 16 tiles of 8 KiB of keys at most: 1024 keys of 64 bf16 dims, 2048 of e4m3; a window of w can touch w + 15
+    assert query(max_keys=1024) == 0 and query(max_keys=1040) > 0
+    assert query(max_keys=2048, cache_dtype=abi.TH_F8E4M3) == 0
+    assert query(window=1009) == 0 and query(window=1010) > 0
+    assert ops.paged_attention_workspace_bytes(4, 8, 2, 64, 4096) == query()
+    with pytest.raises(abi.HipBackendError):
+        ops.paged_attention_workspace_bytes(4, 8, 3, 64, 4096)
 
 
 # ------------------------------------------------------------------ refusals of the Python layer

@@ -305,12 +305,12 @@ def attention64(q, kc, vc, table, pos, rows, scale, window=0, softcap=0.0, slope
 
 
 def check_attention(gpu, lens, hq, hk, d, ps, *, cache=BF16, rows=None, window=0, softcap=0.0, slopes=False, seed=0,
-                    head_major=False, poison=True, amplitude=1.0):
+                    head_major=False, poison=True, amplitude=1.0, row_pages=0):
     from torch_helion.hip import ops
 
     g = gen(seed + 17 * d + ps)
     t, n_rows = len(lens), (len(lens) if rows is None else max(rows) + 1)
-    width = max(1, -(-max(lens) // ps))
+    width = max(1, -(-max(lens) // ps), row_pages)
     kc, vc, table = paged(n_rows, width, ps, hk, d, cache, g, gpu, head_major=head_major)
     pos = torch.tensor(lens, dtype=torch.int32) - 1
     rt = None if rows is None else torch.tensor(rows, dtype=torch.int32)
@@ -388,6 +388,22 @@ def test_attention_outside_the_table(gpu):
     ref, mag, err = attention64(q.view(6, hq, d), kc.float().cpu(), vc.float().cpu(), table.cpu(), pos, rows, 0.125)
     assert_within(out.view(6, hq, d), ref, u(BF16) * (ref.abs() + mag) * (1 + 2 * u(BF16)) + 2 * err * mag + 1e-30)
     assert (out[2:] == 0).all() and (out[:2] != 0).any(1).all()
+
+
+@pytest.mark.parametrize("lens,hq,hk,d,ps,cache", [
+    ([1], 32, 8, 128, 16, BF16), ([0, 0, 0], 4, 2, 64, 32, BF16), ([301], 32, 8, 128, 16, E4M3), ([1, 0, 17, 640, 0], 12, 4, 64, 64, E4M3),
+    ([5] * 300, 3, 1, 64, 16, BF16), ([1000, 31, 33] * 30, 16, 16, 128, 32, BF16), ([700, 650], 40, 2, 128, 16, BF16)])
+def test_attention_short_rows_in_long_tables(gpu, lens, hq, hk, d, ps, cache):
+    """Tables with room for 8192 keys take the line form whatever the lengths: fewer tiles than waves, tokens
+    without keys first, last and between, more tokens than a workgroup has threads' runs of one."""
+    announce(f"paged attention, long tables, lens={lens[:6]} hq={hq} hk={hk} d={d} ps={ps} {cache}")
+    check_attention(gpu, lens, hq, hk, d, ps, cache=cache, row_pages=8192 // ps, poison=len(lens) < 100)
+
+
+def test_attention_many_tokens_of_one_row(gpu):
+    """700 tokens of one row (a prompt's tail): several tokens to each run of the line's prefix sums."""
+    announce("paged attention, 700 tokens of a row")
+    check_attention(gpu, list(range(200, 900)), 2, 1, 64, 64, rows=[0] * 700, row_pages=32)
 
 
 def test_attention_extreme_scores(gpu):
@@ -479,22 +495,23 @@ def test_copy_pages_skips_what_lies_outside(gpu):
 
 
 # ------------------------------------------------------------------ together, captured
-def test_append_and_attention_in_a_graph(gpu):
+@pytest.mark.parametrize("row_pages", [8, 40])
+def test_append_and_attention_in_a_graph(gpu, row_pages):
     """A decode step captured once and replayed with new positions, tokens and page tables, other work
     between the replays: each replay gives the eager calls' bits."""
     from torch_helion.hip import ops
 
-    announce("paged step in a graph")
+    announce(f"paged step in a graph, rows of {row_pages} pages")
     n, hq, hk, d, ps = 5, 8, 2, 128, 16
     g = gen(11)
-    kc, vc, table = paged(n, 8, ps, hk, d, BF16, g, gpu)
+    kc, vc, table = paged(n, row_pages, ps, hk, d, BF16, g, gpu)
     k2, v2 = kc.clone(), vc.clone()
     f = ops.rope_frequencies(d, 10000.0, device=gpu)
     qkv = torch.zeros(n, (hq + 2 * hk) * d, device=gpu)
     pos = torch.zeros(n, dtype=torch.int32, device=gpu)
     q_out = torch.zeros(n, hq * d, dtype=BF16, device=gpu)
     out, q2, out2 = torch.zeros_like(q_out), torch.zeros_like(q_out), torch.zeros_like(q_out)
-    ws = torch.empty(max(ops.paged_attention_workspace_bytes(n, hq, hk, d), 16), dtype=torch.uint8, device=gpu)
+    ws = torch.empty(max(ops.paged_attention_workspace_bytes(n, hq, hk, d, row_pages * ps), 16), dtype=torch.uint8, device=gpu)
 
     def step(kc, vc, q_out, out, ws):
         q, k, v = qkv.split([hq * d, hk * d, hk * d], 1)

@@ -596,8 +596,19 @@ static int line_grid() { return device_cus() > 0 ? device_cus() : 256; }
 
 using namespace th;
 
-extern "C" int64_t th_paged_attention_workspace_bytes(int32_t tokens, int32_t heads_q, int32_t heads_kv, int32_t head_dim) {
-  if (tokens < 0 || heads_q <= 0 || heads_kv <= 0 || heads_q % heads_kv || (head_dim != 64 && head_dim != 128)) return -1;
+// Whether the pairs are so short that each takes one workgroup: the most tiles
+// that one can have by its table and window are 16, four for each wave.
+static bool pair_form(int64_t max_keys, int window, int row_bytes) {
+  const int64_t keys = window ? std::min<int64_t>(max_keys, (int64_t)window + 15) : max_keys;
+  return cdiv(keys * row_bytes, 8192) <= 16;
+}
+
+extern "C" int64_t th_paged_attention_workspace_bytes(int32_t tokens, int32_t heads_q, int32_t heads_kv, int32_t head_dim,
+                                                       int32_t cache_dtype, int64_t max_keys, int32_t window) {
+  if (tokens < 0 || heads_q <= 0 || heads_kv <= 0 || heads_q % heads_kv || (head_dim != 64 && head_dim != 128) ||
+      (cache_dtype != TH_BF16 && cache_dtype != TH_F8E4M3) || max_keys <= 0 || max_keys >= (int64_t)1 << 30 || window < 0)
+    return -1;
+  if (tokens == 0 || pair_form(max_keys, window, head_dim * (cache_dtype == TH_BF16 ? 2 : 1))) return 0;
   const int64_t gq = std::min(heads_q / heads_kv, 16), slots = (int64_t)line_grid() * kLineWaves * 2;
   return cdiv((int64_t)(tokens + 1) * 8, 16) * 16 + cdiv(slots * gq * 2 * 4, 16) * 16 + slots * gq * head_dim * 4;
 }
@@ -639,7 +650,8 @@ extern "C" int th_paged_attention(const th_paged_attn_desc* d, void* stream) {
                d->tokens, d->n_rows);
   TH_CHECK_ARG(d->q && d->k_cache && d->v_cache && d->o && d->positions && d->page_table,
                "th_paged_attention: null tensor pointer");
-  const int64_t need = th_paged_attention_workspace_bytes(d->tokens, d->heads_q, d->heads_kv, d->head_dim);
+  const int64_t need = th_paged_attention_workspace_bytes(
+      d->tokens, d->heads_q, d->heads_kv, d->head_dim, d->cache_dtype, (int64_t)d->row_pages * d->page_size, d->window);
   TH_CHECK_ARG(need == 0 || (d->workspace && ((uintptr_t)d->workspace & 15) == 0 && d->workspace_bytes >= need),
                "th_paged_attention: workspace %lld < %lld bytes, or not 16-byte aligned", (long long)d->workspace_bytes,
                (long long)need);
@@ -669,11 +681,8 @@ extern "C" int th_paged_attention(const th_paged_attn_desc* d, void* stream) {
   k.part = (float*)ws;
   hipStream_t s = (hipStream_t)stream;
   const bool e4 = d->cache_dtype == TH_F8E4M3;
-  // The most tiles that a pair can have, by its table and window: up to 16 of them
-  // (four for each wave) take the pair form.
-  const int64_t keys = std::min<int64_t>((int64_t)d->row_pages * d->page_size, d->window ? (int64_t)d->window + 15 : INT64_MAX);
-  const int64_t pairs = (int64_t)d->tokens * d->heads_kv * k.nqb;
-  if (cdiv(keys * d->head_dim * es, 8192) <= 16 && pairs < (int64_t)1 << 31) {
+  const int64_t pairs = (int64_t)d->tokens * d->heads_kv * k.nqb;  // below 2^24
+  if (pair_form((int64_t)d->row_pages * d->page_size, d->window, (int)(d->head_dim * es))) {
     const dim3 g((unsigned)pairs), b(64 * kPairWaves);
     if (d->head_dim == 128) {
       if (e4) hipLaunchKernelGGL((paged_attn_kernel<128, true, true>), g, b, 0, s, k);

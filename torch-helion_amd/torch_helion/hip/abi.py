@@ -213,7 +213,7 @@ SIGNATURES: dict[str, tuple] = {
     "th_attention_decode": (_i32, [C.POINTER(DecodeDesc), _p]),
     "th_rope": (_i32, [C.POINTER(RopeDesc), _p]),
     "th_paged_append": (_i32, [C.POINTER(PagedAppendDesc), _p]),
-    "th_paged_attention_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32]),
+    "th_paged_attention_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i64, _i32]),
     "th_paged_attention": (_i32, [C.POINTER(PagedAttnDesc), _p]),
     "th_page_copy": (_i32, [C.POINTER(PageCopyDesc), _p]),
     "th_epilogue_vm": (_i32, [C.POINTER(VmDesc), _p]),

@@ -9,6 +9,7 @@ library is missing or the device is not gfx950 they raise
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 from dataclasses import dataclass, field
 from typing import Sequence
@@ -286,43 +287,46 @@ def _refuse(entry: str, message: str) -> None:
     raise abi.HipBackendError(entry, abi.TH_ERR_INVALID, message)
 
 
-def _launch(entry: str, desc: C.Structure, device: torch.device, kernel: str | None) -> None:
-    """One library call on the current stream of ``device``, whichever device is current."""
-    if device.type != "cuda":
-        _refuse("device", f"tensor on {device}, expected a HIP device")
-    if torch._C._cuda_getDevice() != device.index:
-        with torch.cuda.device(device):
-            return _launch(entry, desc, device, kernel)
-    lib = abi.init_device(device.index)
-    status = getattr(lib, entry)(C.byref(desc), torch._C._cuda_getCurrentRawStream(device.index))
+def _launch(entry: str, desc: C.Structure, dev: int, kernel: str | None) -> None:
+    """One library call on the current stream of device ``dev`` (a tensor's get_device()), whichever
+    device is current."""
+    if dev < 0:
+        _refuse("device", "tensors on the CPU, expected a HIP device")
+    if torch._C._cuda_getDevice() != dev:
+        with torch.cuda.device(dev):
+            return _launch(entry, desc, dev, kernel)
+    lib = abi.init_device(dev)
+    status = getattr(lib, entry)(C.byref(desc), torch._C._cuda_getCurrentRawStream(dev))
     if status != abi.TH_OK:
         abi.check(status, entry, kernel)
 
 
-def _vector(t: torch.Tensor, n: int, dtype: torch.dtype, device: torch.device, entry: str, name: str) -> int:
-    """Pointer of n contiguous values on ``device``."""
-    if t.dtype is not dtype or t.numel() != n or not t.is_contiguous() or t.device != device:
-        _refuse(entry, f"{name} must be {n} contiguous {dtype} values on {device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+def _place(dev: int) -> str:
+    return "the CPU" if dev < 0 else f"device {dev}"
+
+
+def _vector(t: torch.Tensor, n: int, dtype: torch.dtype, dev: int, entry: str, name: str) -> int:
+    """Pointer of n contiguous values on device ``dev``."""
+    if t.dtype is not dtype or t.numel() != n or t.get_device() != dev or not t.is_contiguous():
+        _refuse(entry, f"{name} must be {n} contiguous {dtype} values on {_place(dev)}, got {tuple(t.shape)} {t.dtype} on {t.device}")
     return t.data_ptr()
 
 
-def _scales(t: torch.Tensor | None, n: int, device: torch.device, entry: str, name: str) -> int | None:
-    return None if t is None else _vector(t, n, torch.float32, device, entry, name)
-
-
-def _rows_of(t: torch.Tensor, n: int, width: int, dtype: torch.dtype, device: torch.device, entry: str, name: str) -> tuple[int, int]:
-    """(pointer, row stride) of a row-major [n, width] tensor on ``device``."""
-    if t.dtype is not dtype or t.shape != (n, width) or (width != 1 and t.stride(1) != 1) or t.device != device:
-        _refuse(entry, f"{name} must be a row-major [{n}, {width}] {dtype} tensor on {device}, got {tuple(t.shape)} strides "
-                       f"{t.stride()} {t.dtype} on {t.device}")
-    return t.data_ptr(), t.stride(0) if n > 1 else width
+def _rows_of(t: torch.Tensor, n: int, width: int, dtype: torch.dtype, dev: int, entry: str, name: str) -> tuple[int, int]:
+    """(pointer, row stride) of a row-major [n, width] tensor on device ``dev``."""
+    strides = t.stride()
+    if t.dtype is not dtype or t.shape != (n, width) or (strides[1] != 1 and width != 1) or t.get_device() != dev:
+        _refuse(entry, f"{name} must be a row-major [{n}, {width}] {dtype} tensor on {_place(dev)}, got {tuple(t.shape)} strides "
+                       f"{strides} {t.dtype} on {t.device}")
+    return t.data_ptr(), strides[0] if n > 1 else width
 
 
 def _heads(t: torch.Tensor, head_dim: int, entry: str, name: str) -> tuple[int, int]:
     """(tokens, width) of a [tokens, heads * head_dim] tensor."""
-    if t.dim() != 2 or head_dim <= 0 or t.shape[1] % head_dim:
-        _refuse(entry, f"{name} {tuple(t.shape)} is no [tokens, heads * {head_dim}] tensor")
-    return t.shape[0], t.shape[1]
+    shape = t.shape
+    if len(shape) != 2 or head_dim <= 0 or shape[1] % head_dim:
+        _refuse(entry, f"{name} {tuple(shape)} is no [tokens, heads * {head_dim}] tensor")
+    return shape
 
 
 def rope_frequencies(rot_dim: int, theta: float, *, scaling: str | None = None, factor: float = 1.0,
@@ -371,7 +375,7 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, out: tor
     not overlap."""
     entry = "th_rope"
     n, width = _heads(x, head_dim, entry, "x")
-    dev, dt = x.device, x.dtype
+    dev, dt = x.get_device(), x.dtype
     if positions.dtype not in (torch.int32, torch.int64):
         _refuse(entry, f"positions are int32 or int64, got {positions.dtype}")
     half = freqs.numel()
@@ -384,24 +388,25 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, out: tor
     return out
 
 
-def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, device: torch.device, entry: str) -> tuple:
-    """(shape, strides of k, strides of v) of one layer's caches on ``device``."""
+def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, dev: int, entry: str) -> tuple:
+    """(shape, strides of k, strides of v) of one layer's caches on device ``dev``."""
     shape, ks, vs = k_cache.shape, k_cache.stride(), v_cache.stride()
     if len(shape) != 4 or v_cache.shape != shape or v_cache.dtype is not k_cache.dtype:
         _refuse(entry, "k and v caches must be [pages, page_size, heads_kv, head_dim] of one shape and dtype")
     if ks[3] != 1 or vs[3] != 1:
         _refuse(entry, "the head_dim axis of the caches must be contiguous")
-    if k_cache.device != device or v_cache.device != device:
-        _refuse(entry, f"the caches must be on {device}")
+    if k_cache.get_device() != dev or v_cache.get_device() != dev:
+        _refuse(entry, f"the caches must be on {_place(dev)}")
     return shape, ks, vs
 
 
-def _table(page_table: torch.Tensor, device: torch.device, entry: str) -> tuple[int, int, int, int]:
-    """(rows, pages per row, pointer, row stride) of a page table on ``device``."""
-    if page_table.dtype is not torch.int32 or page_table.dim() != 2:
-        _refuse(entry, "page_table must be int32 [rows, pages per row]")
-    rows, width = page_table.shape
-    return (rows, width) + _rows_of(page_table, rows, width, torch.int32, device, entry, "page_table")
+def _table(page_table: torch.Tensor, dev: int, entry: str) -> tuple[int, int, int, int]:
+    """(rows, pages per row, pointer, row stride) of a page table on device ``dev``."""
+    shape, strides = page_table.shape, page_table.stride()
+    if len(shape) != 2 or page_table.dtype is not torch.int32 or (strides[1] != 1 and shape[1] != 1) or page_table.get_device() != dev:
+        _refuse(entry, f"page_table must be a row-major int32 [rows, pages per row] tensor on {_place(dev)}")
+    rows, width = shape
+    return rows, width, page_table.data_ptr(), strides[0] if rows > 1 else width
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -420,7 +425,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, k_ca
     outside the table or the cache is left out and counted in ``n_invalid`` (an int32 device
     scalar that the caller zeroes). Two tokens of a call must not share a slot."""
     entry = "th_paged_append"
-    n, dev, dt = k.shape[0], k.device, k.dtype
+    n, dev, dt = k.shape[0], k.get_device(), k.dtype
     (pages, page_size, hk, hd), ks, vs = _cache(k_cache, v_cache, dev, entry)
     n_rows, row_pages, tp, ldt = _table(page_table, dev, entry)
     pos = _vector(positions, n, torch.int32, dev, entry, "positions")
@@ -443,16 +448,27 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, k_ca
         n, hq, hk, hd, 2 * half, interleaved, th_dtype(dt), th_dtype(k_cache.dtype), page_size, n_rows, row_pages, pages,
         rope_scale, 0, pos, rp, tp, ldt, fp, qp, ldq, op, ldo, kp, ldk, vp, ldv,
         k_cache.data_ptr(), ks[0], ks[1], ks[2], v_cache.data_ptr(), vs[0], vs[1], vs[2],
-        _scales(k_scale, hk, dev, entry, "k_scale"), _scales(v_scale, hk, dev, entry, "v_scale"),
+        None if k_scale is None else _vector(k_scale, hk, torch.float32, dev, entry, "k_scale"), None if v_scale is None else _vector(v_scale, hk, torch.float32, dev, entry, "v_scale"),
         None if n_invalid is None else _vector(n_invalid, 1, torch.int32, dev, entry, "n_invalid"))
     _launch(entry, d, dev, kernel)
 
 
-def paged_attention_workspace_bytes(tokens: int, heads_q: int, heads_kv: int, head_dim: int) -> int:
-    n = abi.load().th_paged_attention_workspace_bytes(tokens, heads_q, heads_kv, head_dim)
+@functools.lru_cache(maxsize=1024)
+def _paged_workspace(dev: int, tokens: int, heads_q: int, heads_kv: int, head_dim: int, max_keys: int, window: int,
+                     dtype: torch.dtype) -> int:
+    lib = abi.load() if dev < 0 else abi.init_device(dev)
+    n = lib.th_paged_attention_workspace_bytes(tokens, heads_q, heads_kv, head_dim, th_dtype(dtype), max_keys, window)
     if n < 0:
-        _refuse("th_paged_attention_workspace_bytes", f"tokens={tokens} heads_q={heads_q} heads_kv={heads_kv} head_dim={head_dim}")
+        _refuse("th_paged_attention_workspace_bytes", f"tokens={tokens} heads_q={heads_q} heads_kv={heads_kv} "
+                                                      f"head_dim={head_dim} max_keys={max_keys} window={window} {dtype}")
     return int(n)
+
+
+def paged_attention_workspace_bytes(tokens: int, heads_q: int, heads_kv: int, head_dim: int, max_keys: int, *, window: int = 0,
+                                    dtype: torch.dtype = torch.bfloat16) -> int:
+    """Workspace of :func:`paged_attention` over a cache of ``dtype`` whose page table has room for
+    ``max_keys`` keys a row (pages per row * page_size). 0 where it needs none."""
+    return _paged_workspace(-1, tokens, heads_q, heads_kv, head_dim, max_keys, window, dtype)
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
@@ -469,7 +485,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``workspace``: :func:`paged_attention_workspace_bytes` bytes that no concurrent call uses;
     without one the call takes it from torch's allocator."""
     entry = "th_paged_attention"
-    dev = q.device
+    dev = q.get_device()
     (pages, page_size, hk, hd), ks, vs = _cache(k_cache, v_cache, dev, entry)
     n, width = _heads(q, hd, entry, "q")
     n_rows, row_pages, tp, ldt = _table(page_table, dev, entry)
@@ -478,18 +494,21 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     hq = width // hd
     qp, ldq = _rows_of(q, n, width, torch.bfloat16, dev, entry, "q")
     op, ldo = _rows_of(out, n, width, torch.bfloat16, dev, entry, "out")
-    sp = _scales(slopes, hq, dev, entry, "slopes")
-    if workspace is None:
-        if dev.type == "cuda":
-            abi.init_device(dev.index)
-            workspace = torch.empty(paged_attention_workspace_bytes(n, hq, hk, hd), dtype=torch.uint8, device=dev)
-    elif workspace.device != dev or not workspace.is_contiguous():
-        _refuse(entry, f"workspace must be a contiguous tensor on {dev}")
-    wp, wn = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    sp = None if slopes is None else _vector(slopes, hq, torch.float32, dev, entry, "slopes")
+    wp, wn = None, 0
+    if workspace is not None:
+        if workspace.get_device() != dev or not workspace.is_contiguous():
+            _refuse(entry, f"workspace must be a contiguous tensor on {_place(dev)}")
+        wp, wn = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    elif dev >= 0:
+        wn = _paged_workspace(dev, n, hq, hk, hd, row_pages * page_size, window, k_cache.dtype)
+        if wn:
+            workspace = torch.empty(wn, dtype=torch.uint8, device=q.device)
+            wp = workspace.data_ptr()
     d = abi.PagedAttnDesc(
         n, hq, hk, hd, th_dtype(k_cache.dtype), page_size, n_rows, row_pages, pages, window, scale, softcap, 0, pos, rp, tp, ldt,
         qp, ldq, k_cache.data_ptr(), ks[0], ks[1], ks[2], v_cache.data_ptr(), vs[0], vs[1], vs[2],
-        sp, _scales(k_scale, hk, dev, entry, "k_scale"), _scales(v_scale, hk, dev, entry, "v_scale"), op, ldo, wp, wn)
+        sp, None if k_scale is None else _vector(k_scale, hk, torch.float32, dev, entry, "k_scale"), None if v_scale is None else _vector(v_scale, hk, torch.float32, dev, entry, "v_scale"), op, ldo, wp, wn)
     _launch(entry, d, dev, kernel)
     return out
 
@@ -504,19 +523,21 @@ def copy_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, src: torch.Tensor, 
     to ``page_map[p]`` in the same launch: a move. Pairs and entries outside the cache are left
     alone. No page may be both a source and a destination, or twice a destination."""
     entry = "th_page_copy"
-    shape, dev = k_cache.shape, k_cache.device
-    if len(shape) not in (4, 5) or v_cache.shape != shape or v_cache.dtype is not k_cache.dtype or v_cache.device != dev:
+    shape, dev = k_cache.shape, k_cache.get_device()
+    if len(shape) not in (4, 5) or v_cache.shape != shape or v_cache.dtype is not k_cache.dtype or v_cache.get_device() != dev:
         _refuse(entry, "k and v caches must be [layers, pages, page_size, heads_kv, head_dim] of one shape, dtype and device")
     size, n = k_cache.element_size(), src.numel()
     layered, pages = len(shape) == 5, shape[-4]
     page = shape[-3] * shape[-2] * shape[-1] * size
     operands = []
     for t, name in ((k_cache, "k"), (v_cache, "v")):
-        strides, run = t.stride(), 1
-        for stride, extent in sorted(zip(strides[-3:], shape[-3:])):
-            if extent != 1 and stride != run:
-                _refuse(entry, f"a page of the {name} cache must be one dense block, got strides {strides}")
-            run *= extent
+        strides = t.stride()
+        if strides[-3:] != (shape[-2] * shape[-1], shape[-1], 1):   # else some other order of one dense block
+            run = 1
+            for stride, extent in sorted(zip(strides[-3:], shape[-3:])):
+                if extent != 1 and stride != run:
+                    _refuse(entry, f"a page of the {name} cache must be one dense block, got strides {strides}")
+                run *= extent
         operands += [t.data_ptr(), strides[0] * size if layered else 0, strides[-4] * size]
     table = (None, 0, 0, 0, None)
     if page_table is not None:
