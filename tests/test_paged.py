@@ -235,3 +235,108 @@ def test_more_argument_checks():
             (copy, {"k_cache": a["k_cache"][:, ::2], "v_cache": a["v_cache"][:, ::2]}, "dense"), (copy, {}, "HIP device")):
         with pytest.raises(abi.HipBackendError, match=message):
             call(**kw)
+
+
+# ------------------------------------------------------------------ who holds which page
+def page_book(**kw):
+    from torch_helion.hip.paged import PageBook
+
+    return PageBook(**{**dict(pages=12, page_size=4, rows=4, row_pages=6), **kw})
+
+
+def snapshot(book):
+    return (list(book.refs), sorted(book.free), sorted(book.free_rows), {r: list(p) for r, p in book.pages.items()}, dict(book.length))
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_page_book_against_token_lists(seed):
+    """Random opens, forks, extensions, cuts, closes and compactions: every row reads back its own
+    tokens from the pages it is said to hold, and the counts add up; a refused call changes nothing."""
+    import random
+
+    from torch_helion.hip import abi
+
+    rng = random.Random(seed)
+    book = page_book(pages=rng.choice([5, 12, 30]), page_size=rng.choice([1, 4, 16]))
+    content = {p: [None] * book.page_size for p in range(len(book.refs))}
+    tokens: dict[int, list[int]] = {}
+    stamp, refused = 0, 0
+    for _ in range(400):
+        act = rng.choice(["open", "fork", "extend", "extend", "extend", "extend", "shrink", "close", "compact"])
+        before = snapshot(book)
+        rows = list(tokens)
+        try:
+            if act == "open":
+                tokens[book.open()] = []
+            elif act == "fork" and rows:
+                r = rng.choice(rows)
+                tokens[book.fork(r)] = list(tokens[r])
+            elif act == "extend" and rows:
+                counts = {r: rng.choice([0, 1, 1, 1, rng.randint(2, 9)]) for r in rng.sample(rows, rng.randint(1, len(rows)))}
+                copies, entries = book.extend(counts)
+                table = {(r, i): p for r, i, p in entries}
+                for a, b in copies:
+                    content[b] = list(content[a])
+                for r, n in counts.items():
+                    for i in range(n):
+                        stamp += 1
+                        at = len(tokens[r]) // book.page_size
+                        page = book.pages[r][at]
+                        assert table.get((r, at), page) == page and book.refs[page] == 1
+                        content[page][len(tokens[r]) % book.page_size] = stamp
+                        tokens[r].append(stamp)
+            elif act == "shrink" and rows:
+                r = rng.choice(rows)
+                n = rng.randint(0, len(tokens[r]))
+                book.shrink(r, n)
+                del tokens[r][n:]
+            elif act == "close" and rows:
+                r = rng.choice(rows)
+                book.close(r)
+                del tokens[r]
+            elif act == "compact":
+                moves = book.compact()
+                assert not {a for a, _ in moves} & {b for _, b in moves}
+                for a, b in moves:
+                    content[b] = list(content[a])
+                used = sum(r > 0 for r in book.refs)
+                assert all(r > 0 for r in book.refs[:used]) and not any(book.refs[used:])
+        except abi.HipBackendError:
+            refused += 1
+            assert snapshot(book) == before
+        for r, want in tokens.items():
+            assert book.length[r] == len(want) and len(book.pages[r]) == -(-len(want) // book.page_size)
+            got = [content[p][i] for p in book.pages[r] for i in range(book.page_size)][:len(want)]
+            assert got == want
+        held = [p for pages in book.pages.values() for p in pages]
+        assert [held.count(p) for p in range(len(book.refs))] == book.refs
+        assert sorted(book.free) == [p for p, n in enumerate(book.refs) if n == 0] and len(set(held) & set(book.free)) == 0
+    assert refused > 0
+
+
+def test_page_book_refusals():
+    from torch_helion.hip import abi
+    from torch_helion.hip.paged import PagedKVCache
+
+    book = page_book(pages=3, page_size=4, rows=2, row_pages=2)
+    row = book.open()
+    for call, message in ((lambda: book.extend({row: 9}), "exceed the table"), (lambda: book.extend({5: 1}), "not open"),
+                          (lambda: book.extend({row: -1}), "tokens"), (lambda: book.fork(7), "not open"), (lambda: book.close(7), "not open"),
+                          (lambda: book.shrink(row, 1), "tokens")):
+        with pytest.raises(abi.HipBackendError, match=message):
+            call()
+    book.extend({row: 8})
+    other = book.fork(row)
+    with pytest.raises(abi.HipBackendError, match="no free row"):
+        book.open()
+    book.shrink(other, 6)
+    assert book.extend({other: 1}) == ([(1, 2)], [(other, 1, 2)])       # its last page was shared
+    book.close(row)
+    row = book.open()
+    with pytest.raises(abi.HipBackendError, match="pages needed"):
+        book.extend({row: 5})
+    assert book.length[row] == 0 and book.free == [1]
+    sizes = dict(layers=1, pages=4, page_size=16, kv_heads=1, head_dim=64, rows=1, max_len=64)
+    for change, message in (({"device": "cpu"}, "HIP device"),):
+        with pytest.raises(abi.HipBackendError, match=message):
+            PagedKVCache(**{**sizes, **change})

@@ -102,8 +102,6 @@ class DecodeBlock:
         self.g1 = g1.to(dev).contiguous()
         self.g2 = g2.to(dev).contiguous()
         bf = torch.bfloat16
-        self.k_cache = torch.zeros(B, max_len, kv_heads, self.hd, dtype=bf, device=dev)
-        self.v_cache = torch.zeros_like(self.k_cache)
         self.q = torch.empty(B, heads * self.hd, dtype=bf, device=dev)
         self.attn = torch.empty_like(self.q)
         self.x1 = torch.empty(B, hidden, dtype=bf, device=dev)  # with fold_gain: bf16(x1) g2
@@ -113,15 +111,22 @@ class DecodeBlock:
         self.act = torch.empty(B, intermediate, dtype=bf, device=dev)
         self.out = torch.empty(B, hidden, dtype=bf, device=dev)
         self.out32 = torch.empty(B, hidden, device=dev)
-        inv = 1.0 / (rope_theta ** (torch.arange(0, self.hd, 2, dtype=torch.float64) / self.hd))
+        ws = max(ops.gemm_workspace_bytes(B, p.n, p.k, p.n_acc, _FP8) for p in (self.wqkv, self.wo, self.wgu, self.wd))
+        self.gemm_ws = torch.empty(max(ws, 16), dtype=torch.uint8, device=dev)
+        self.graph: torch.cuda.CUDAGraph | None = None
+        self._allocate_cache()
+
+    def _allocate_cache(self) -> None:
+        """The contiguous caches, the RoPE rows of their positions and the attention's workspace."""
+        dev, B, max_len = self.device, self.B, self.max_len
+        self.k_cache = torch.zeros(B, max_len, self.Hkv, self.hd, dtype=torch.bfloat16, device=dev)
+        self.v_cache = torch.zeros_like(self.k_cache)
+        inv = 1.0 / (self.theta ** (torch.arange(0, self.hd, 2, dtype=torch.float64) / self.hd))
         ang = torch.outer(torch.arange(max_len, dtype=torch.float64), inv)
         ang = torch.cat([ang, ang], -1)
         self.cos = ang.cos().float().to(dev).contiguous()
         self.sin = ang.sin().float().to(dev).contiguous()
-        ws = max(ops.gemm_workspace_bytes(B, p.n, p.k, p.n_acc, _FP8) for p in (self.wqkv, self.wo, self.wgu, self.wd))
-        self.gemm_ws = torch.empty(max(ws, 16), dtype=torch.uint8, device=dev)
-        self.graph: torch.cuda.CUDAGraph | None = None
-        aw = ops.attention_decode_workspace_bytes(B, heads, kv_heads, self.hd, max_len)
+        aw = ops.attention_decode_workspace_bytes(B, self.H, self.Hkv, self.hd, max_len)
         self.attn_ws = torch.empty(max(aw // 4, 1), device=dev)
 
     # ------------------------------------------------------------------
@@ -156,6 +161,12 @@ class DecodeBlock:
                    rscale_mask=0b1, lhs_gain=self.g1, **norm, **rope)
         ops.attention_decode(self.q, self.k_cache, self.v_cache, self.attn, scale=1.0 / math.sqrt(self.hd),
                              fixed_len=pos + 1, workspace=self.attn_ws)
+        return self._after_attention(x)
+
+    def _after_attention(self, x: torch.Tensor) -> torch.Tensor:
+        """k2 .. k4: the block output from ``self.attn`` and the residual x."""
+        E = abi
+        norm = dict(sumsq=True, inv_k=1.0 / self.D, eps=self.eps)
         o_outs = [ops.EpiSpec(E.EPI_ADD, self.x1, e=0), ops.EpiSpec(E.EPI_ADD, self.x1_32, e=0)]
         gu_outs = [ops.EpiSpec(E.EPI_SWIGLU, self.act, a=0, b=1)]
         if self.fold_gain:
