@@ -182,6 +182,8 @@ def test_workspace_query(lib):
     assert query(max_keys=1024) == 0 and query(max_keys=1040) > 0
     assert query(max_keys=2048, cache_dtype=abi.TH_F8E4M3) == 0
     assert query(window=1009) == 0 and query(window=1010) > 0
+    # up to 32 tiles from 128 pairs on
+    assert query(max_keys=2048, tokens=63) > 0 and query(max_keys=2048, tokens=64) == 0 and query(max_keys=2064, tokens=64) > 0
     assert ops.paged_attention_workspace_bytes(4, 8, 2, 64, 4096) == query()
     with pytest.raises(abi.HipBackendError):
         ops.paged_attention_workspace_bytes(4, 8, 3, 64, 4096)

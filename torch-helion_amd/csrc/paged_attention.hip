@@ -20,9 +20,10 @@
 //            alone, the older half of them is served first and ends at 108 us
 //            where the younger ends at 134 (64 sequences of 2048-4096 keys); and
 //            the heads of a key, neighbours in memory, are read together.
-//   pair     a workgroup of four waves for each pair, its tiles dealt out in turn
-//            and the waves merged in LDS: where a pair can have only a few tiles
-//            by its table and window, one launch and no line to lay out.
+//   pair     a workgroup for each (token, kv head) pair, its tiles dealt out to
+//            the waves in turn and the waves merged in LDS: where a pair can have
+//            only a few tiles by its table and window, one launch and no line to
+//            lay out.
 //
 // One tile:
 //   K        loaded straight in the operand layout of S^T = K Q^T
@@ -147,12 +148,12 @@ struct PaTile {
   static constexpr int LDS = KT * D * 2;        // one wave's V tile, bf16
 };
 
-constexpr int kLineWaves = 8, kPairWaves = 4;  // waves of a workgroup
+constexpr int kLineWaves = 8;
 
-template <int D, bool E4, bool PAIR>
-__global__ void __launch_bounds__(64 * (PAIR ? kPairWaves : kLineWaves), PAIR ? 2 : 1) paged_attn_kernel(PAttnK p) {
+// NW: waves of a workgroup.
+template <int D, bool E4, bool PAIR, int NW>
+__global__ void __launch_bounds__(64 * NW, 8 / NW) paged_attn_kernel(PAttnK p) {
   using T = PaTile<D, E4>;
-  constexpr int NW = PAIR ? kPairWaves : kLineWaves;
   constexpr int KU = PAIR ? NW * T::KT : T::KT;  // keys of a step: of the workgroup's, or of one wave's
   constexpr int RB = T::RB, KT = T::KT, NB = T::NB, CPR = T::CPR, RPI = T::RPI;
   constexpr int NKS = D / 32, NDB = D / 16, JPR = RB / 64;  // JPR: K loads per 16-key block
@@ -589,6 +590,24 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(PAttnK p, int wave
   for (int r = 0; r < 4; ++r) o[c * D + 4 * ln + r] = f32_to_bf16(x[r] * f);
 }
 
+template <int D, bool E4>
+static void launch_paged_as(const PAttnK& k, bool pair, int waves, unsigned grid, hipStream_t s) {
+  const dim3 g(grid), b(64 * waves);
+  if (!pair) hipLaunchKernelGGL((paged_attn_kernel<D, E4, false, kLineWaves>), g, b, 0, s, k);
+  else if (waves == 8) hipLaunchKernelGGL((paged_attn_kernel<D, E4, true, 8>), g, b, 0, s, k);
+  else hipLaunchKernelGGL((paged_attn_kernel<D, E4, true, 4>), g, b, 0, s, k);
+}
+
+static void launch_paged(const PAttnK& k, int head_dim, bool e4, bool pair, int waves, unsigned grid, hipStream_t s) {
+  if (head_dim == 128) {
+    if (e4) launch_paged_as<128, true>(k, pair, waves, grid, s);
+    else launch_paged_as<128, false>(k, pair, waves, grid, s);
+  } else {
+    if (e4) launch_paged_as<64, true>(k, pair, waves, grid, s);
+    else launch_paged_as<64, false>(k, pair, waves, grid, s);
+  }
+}
+
 // One workgroup of eight waves per CU.
 static int line_grid() { return device_cus() > 0 ? device_cus() : 256; }
 
@@ -596,20 +615,31 @@ static int line_grid() { return device_cus() > 0 ? device_cus() : 256; }
 
 using namespace th;
 
-// Whether the pairs are so short that each takes one workgroup: the most tiles
-// that one can have by its table and window are 16, four for each wave.
-static bool pair_form(int64_t max_keys, int window, int row_bytes) {
+// The most tiles that a pair can have, by its table and window.
+static int64_t most_tiles(int64_t max_keys, int window, int row_bytes) {
   const int64_t keys = window ? std::min<int64_t>(max_keys, (int64_t)window + 15) : max_keys;
-  return cdiv(keys * row_bytes, 8192) <= 16;
+  return cdiv(keys * row_bytes, 8192);
 }
+
+// Whether pairs take the pair form. In a graph, us, pair against line form, lengths
+// of half to all of the room (bf16, 128 dims, 8 kv heads, 4 query heads each):
+//   tiles of room      16            32            64
+//     8 pairs       9.8 /  9.8   14.5 / 10.6   23.6 / 10.5
+//   128 pairs      10.8 / 15.0   16.2 / 20.9   26.2 / 29.0
+//   512 pairs      20.4 / 28.8   42.0 / 50.0   80.1 / 85.4
+//  2048 pairs      79.3 / 92.8    147 /  160    286 /  288
+// 64 tiles and more stay with the line: lengths are not known here, and one full
+// row among short ones would cost the pair form 24 us where the line takes 10.
+static bool pair_form(int64_t tiles, int64_t pairs) { return tiles <= 16 || (tiles <= 32 && pairs >= 128); }
 
 extern "C" int64_t th_paged_attention_workspace_bytes(int32_t tokens, int32_t heads_q, int32_t heads_kv, int32_t head_dim,
                                                        int32_t cache_dtype, int64_t max_keys, int32_t window) {
   if (tokens < 0 || heads_q <= 0 || heads_kv <= 0 || heads_q % heads_kv || (head_dim != 64 && head_dim != 128) ||
       (cache_dtype != TH_BF16 && cache_dtype != TH_F8E4M3) || max_keys <= 0 || max_keys >= (int64_t)1 << 30 || window < 0)
     return -1;
-  if (tokens == 0 || pair_form(max_keys, window, head_dim * (cache_dtype == TH_BF16 ? 2 : 1))) return 0;
-  const int64_t gq = std::min(heads_q / heads_kv, 16), slots = (int64_t)line_grid() * kLineWaves * 2;
+  const int g = heads_q / heads_kv, row_bytes = head_dim * (cache_dtype == TH_BF16 ? 2 : 1);
+  if (tokens == 0 || pair_form(most_tiles(max_keys, window, row_bytes), tokens * heads_kv * cdiv(g, 16))) return 0;
+  const int64_t gq = std::min(g, 16), slots = (int64_t)line_grid() * kLineWaves * 2;
   return cdiv((int64_t)(tokens + 1) * 8, 16) * 16 + cdiv(slots * gq * 2 * 4, 16) * 16 + slots * gq * head_dim * 4;
 }
 
@@ -682,26 +712,16 @@ extern "C" int th_paged_attention(const th_paged_attn_desc* d, void* stream) {
   hipStream_t s = (hipStream_t)stream;
   const bool e4 = d->cache_dtype == TH_F8E4M3;
   const int64_t pairs = (int64_t)d->tokens * d->heads_kv * k.nqb;  // below 2^24
-  if (pair_form((int64_t)d->row_pages * d->page_size, d->window, (int)(d->head_dim * es))) {
-    const dim3 g((unsigned)pairs), b(64 * kPairWaves);
-    if (d->head_dim == 128) {
-      if (e4) hipLaunchKernelGGL((paged_attn_kernel<128, true, true>), g, b, 0, s, k);
-      else hipLaunchKernelGGL((paged_attn_kernel<128, false, true>), g, b, 0, s, k);
-    } else {
-      if (e4) hipLaunchKernelGGL((paged_attn_kernel<64, true, true>), g, b, 0, s, k);
-      else hipLaunchKernelGGL((paged_attn_kernel<64, false, true>), g, b, 0, s, k);
-    }
+  const int64_t tiles = most_tiles((int64_t)d->row_pages * d->page_size, d->window, (int)(d->head_dim * es));
+  if (pair_form(tiles, pairs)) {
+    // eight waves where there is a CU for each pair and they have more than a tile
+    // each (256 pairs, 16 tiles of e4m3: 16.1 us against 16.7, 32 tiles 24.1 against
+    // 27.5), else four (4 tiles 6.2 against 7.0; 512 pairs would wait for CUs)
+    launch_paged(k, d->head_dim, e4, true, pairs <= device_cus() && tiles > 8 ? 8 : 4, (unsigned)pairs, s);
     TH_CHECK_LAUNCH();
     return TH_OK;
   }
-  const dim3 g(grid), b(64 * kLineWaves);
-  if (d->head_dim == 128) {
-    if (e4) hipLaunchKernelGGL((paged_attn_kernel<128, true, false>), g, b, 0, s, k);
-    else hipLaunchKernelGGL((paged_attn_kernel<128, false, false>), g, b, 0, s, k);
-  } else {
-    if (e4) hipLaunchKernelGGL((paged_attn_kernel<64, true, false>), g, b, 0, s, k);
-    else hipLaunchKernelGGL((paged_attn_kernel<64, false, false>), g, b, 0, s, k);
-  }
+  launch_paged(k, d->head_dim, e4, false, kLineWaves, (unsigned)grid, s);
   TH_CHECK_LAUNCH();
   // few pairs: a workgroup for each head, so that their many parts are read at once
   const int hw = pairs >= 256 ? std::min(k.gq, 1024 / d->head_dim) : 1;
