@@ -173,7 +173,7 @@ def paged(rows, row_pages, page_size, hk, d, dtype, g, gpu, spare=3, head_major=
     (32, 8, 128, 128, False, 16, torch.float32, BF16, False), (8, 8, 64, 64, False, 32, torch.bfloat16, BF16, True),
     (4, 1, 128, 64, True, 64, torch.bfloat16, E4M3, False), (0, 4, 64, 0, False, 16, torch.float32, E4M3, True),
     (6, 2, 96, 40, False, 8, torch.bfloat16, BF16, False), (3, 3, 20, 10, True, 1, torch.float32, E4M3, False),
-    (12, 4, 128, 128, False, 256, torch.bfloat16, E4M3, False), (1, 1, 128, 104, False, 32, torch.float32, BF16, False),
+    (12, 4, 128, 128, False, 256, torch.bfloat16, E4M3, False), (5, 2, 64, 0, False, 32, torch.float32, BF16, False), (1, 1, 128, 104, False, 32, torch.float32, BF16, False),
 ])
 def test_append(gpu, hq, hk, d, rot, interleaved, ps, in_dtype, cache, head_major):
     """Ragged prompts, some padded tokens: the slots written, and nothing else."""
@@ -364,6 +364,14 @@ def test_attention_window_cap_and_bias(gpu, window, softcap, slopes, cache):
     check_attention(gpu, [31, 1500], 4, 4, 128, 16, window=window, softcap=softcap, slopes=slopes, cache=cache, amplitude=6.0)
 
 
+@pytest.mark.parametrize("window,softcap,slopes,cache", [(1500, 0.0, False, BF16), (2100, 10.0, True, E4M3), (1030, 0.0, True, BF16)])
+def test_attention_long_windows(gpu, window, softcap, slopes, cache):
+    """Windows of more tiles than the pair form takes, ahead of, at and past the lengths' ends."""
+    announce(f"paged attention long window={window} {cache}")
+    check_attention(gpu, [window - 1, 3000, window, window + 1, 0, window + 16, 2999], 4, 2, 64, 16, window=window, softcap=softcap,
+                    slopes=slopes, cache=cache, amplitude=4.0)
+
+
 def test_attention_rows_and_head_major_pages(gpu):
     """Several tokens of one row (a speculated run), rows in any order, pages laid out head by head."""
     announce("paged attention with rows")
@@ -388,6 +396,12 @@ def test_attention_outside_the_table(gpu):
     ref, mag, err = attention64(q.view(6, hq, d), kc.float().cpu(), vc.float().cpu(), table.cpu(), pos, rows, 0.125)
     assert_within(out.view(6, hq, d), ref, u(BF16) * (ref.abs() + mag) * (1 + 2 * u(BF16)) + 2 * err * mag + 1e-30)
     assert (out[2:] == 0).all() and (out[:2] != 0).any(1).all()
+    # a bias by distance far past the table: the distances' differences are what counts
+    far = torch.full((1,), 2147483647, dtype=torch.int32)
+    slopes = torch.full((hq,), 0.25)
+    ops.paged_attention(q[:1].to(gpu), kc, vc, table, far.to(gpu), out[:1], scale=0.125, slopes=slopes.to(gpu))
+    ref, mag, err = attention64(q[:1].view(1, hq, d), kc.float().cpu(), vc.float().cpu(), table.cpu(), far, None, 0.125, slopes=slopes)
+    assert_within(out[:1].view(1, hq, d), ref, u(BF16) * (ref.abs() + mag) * (1 + 2 * u(BF16)) + 2 * err * mag + 1e-30)
 
 
 @pytest.mark.parametrize("lens,hq,hk,d,ps,cache", [

@@ -81,12 +81,11 @@ __device__ __forceinline__ void pa_lds_order() {
 }
 
 // A token's keys: [lo, hi) of its row; units start at lo rounded down to 16.
-struct Span { int pos, row, lo, hi, base, units; };  // units of KU keys
+struct Span { int row, lo, hi, base, units; };  // units of KU keys
 
 template <int KU>
 __device__ __forceinline__ Span span_from(const PAttnK& p, int pos, int row) {
   Span s;
-  s.pos = pos;
   s.row = row;
   const bool in = row >= 0 && row < p.n_rows && pos >= 0;
   s.hi = in ? (int)min((int64_t)pos + 1, (int64_t)p.row_pages << p.pshift) : 0;
@@ -229,7 +228,7 @@ __global__ void __launch_bounds__(64 * NW, 8 / NW) paged_attn_kernel(PAttnK p) {
     t = run * per;
     int64_t at = pre[run];
     sp = span_of<KU>(p, t);
-    while (at + sp.units <= u0) {
+    while (at + sp.units <= u0 && t < p.tokens - 1) {
       at += sp.units;
       sp = span_of<KU>(p, ++t);
     }
@@ -391,7 +390,7 @@ __global__ void __launch_bounds__(64 * NW, 8 / NW) paged_attn_kernel(PAttnK p) {
         k = 0;
         ++t;
         sp = span_from<KU>(p, __builtin_amdgcn_readfirstlane(npos), p.rows ? __builtin_amdgcn_readfirstlane(nrow) : t);
-        while (sp.units == 0) sp = span_of<KU>(p, ++t);
+        while (sp.units == 0 && t < last_t) sp = span_of<KU>(p, ++t);
         load_next();
         p0 = 1 << 30;
       }
@@ -410,11 +409,11 @@ __global__ void __launch_bounds__(64 * NW, 8 / NW) paged_attn_kernel(PAttnK p) {
           if (cap) x = capl - 2.f * capl * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x));
           s[b][r] = x;
         }
-      if (p.slopes) {
+      if (p.slopes) {  // from the last key: what lies between it and pos is the same for all
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) s[b][r] -= slope * (float)(cs.pos - (j0 + 16 * b + 4 * g + r));
+          for (int r = 0; r < 4; ++r) s[b][r] -= slope * (float)(cs.hi - 1 - (j0 + 16 * b + 4 * g + r));
       }
       if (j0 < cs.lo || j0 + KT > cs.hi || ok != (1u << NB) - 1) {
 #pragma unroll
@@ -674,8 +673,8 @@ extern "C" int th_paged_attention(const th_paged_attn_desc* d, void* stream) {
   TH_CHECK_ARG((!d->k_scale && !d->v_scale) || d->cache_dtype == TH_F8E4M3,
                "th_paged_attention: scales need an e4m3 cache");
   if (d->tokens == 0) return TH_OK;
-  TH_CHECK_ARG(d->heads_kv * cdiv(d->heads_q / d->heads_kv, 16) <= 256,
-               "th_paged_attention: more than 256 kv heads (each 16 query heads of one count)");
+  TH_CHECK_ARG(d->heads_kv * cdiv(d->heads_q / d->heads_kv, 16) <= std::min(256, line_grid() * kLineWaves),
+               "th_paged_attention: more than 256 kv heads (each block of 16 query heads counts)");
   TH_CHECK_ARG(d->rows || d->tokens <= d->n_rows, "th_paged_attention: %d tokens without rows exceed the table's %d",
                d->tokens, d->n_rows);
   TH_CHECK_ARG(d->q && d->k_cache && d->v_cache && d->o && d->positions && d->page_table,

@@ -367,7 +367,7 @@ def rope_frequencies(rot_dim: int, theta: float, *, scaling: str | None = None, 
 def rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, out: torch.Tensor, *, head_dim: int,
          interleaved: bool = False, scale: float = 1.0, inverse: bool = False, kernel: str | None = None) -> torch.Tensor:
     """Rotary positions: every head of x [tokens, heads * head_dim] (bf16 or fp32) has its first
-    ``2 * len(freqs)`` dims turned by the token's own position (int32 or int64 [tokens]; any value).
+    ``2 * len(freqs)`` dims turned by the token's own position (int32 or int64 [tokens]; angles are reduced in 64 bits).
 
     Pairs are dims (i, i + len(freqs)), or (2 i, 2 i + 1) with ``interleaved``; ``scale`` multiplies
     the rotated dims, the others are copied. ``inverse`` turns back: called on the gradient of the
