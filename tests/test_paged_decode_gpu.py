@@ -143,12 +143,12 @@ def test_forks_and_compaction_keep_every_row(gpu):
             for c, w in zip((cache.k, cache.v), want):
                 assert torch.equal(c[layer, pages].reshape(-1, hk * d)[:w.shape[0]].cpu(), w), (r, layer)
 
-    def attend():
+    def attend(**kw):
         live = sorted({r for r, _ in tokens})
         q = torch.randn(len(live), 4 * d, generator=torch.Generator().manual_seed(5)).to(BF16).to(gpu)
         out = torch.empty_like(q)
         cache.attend(1, q, torch.tensor([cache.length(r) - 1 for r in live], dtype=torch.int32, device=gpu), out, scale=0.125,
-                     rows=torch.tensor(live, dtype=torch.int32, device=gpu))
+                     rows=torch.tensor(live, dtype=torch.int32, device=gpu), **kw)
         return out
 
     a, b = cache.open(), cache.open()
@@ -165,6 +165,7 @@ def test_forks_and_compaction_keep_every_row(gpu):
     cache.shrink(forks[1], 17)
     tokens = {(r, layer): w[:, :17] if r == forks[1] else w for (r, layer), w in tokens.items() if r != b}
     out = attend()
+    assert torch.equal(attend(max_keys=60), out)                      # no row is longer: a narrower table, the same keys
     used = 24 - cache.free_pages
     assert cache.compact() == used and int(cache.page_table.max()) == used - 1
     check()

@@ -244,10 +244,17 @@ class PagedKVCache:
         """``ops.paged_append`` on a layer's pages (its ``rows``, ``freqs``, ``q``, ... as options)."""
         ops.paged_append(k, v, positions, self.k[layer], self.v[layer], self.page_table, **self._scales(layer), **options)
 
-    def attend(self, layer: int, q: torch.Tensor, positions: torch.Tensor, out: torch.Tensor, **options) -> torch.Tensor:
-        """``ops.paged_attention`` on a layer's pages (its ``scale``, ``rows``, ``window``, ... as options)."""
-        return ops.paged_attention(q, self.k[layer], self.v[layer], self.page_table, positions, out, **self._scales(layer),
-                                   **options)
+    def attend(self, layer: int, q: torch.Tensor, positions: torch.Tensor, out: torch.Tensor, *, max_keys: int | None = None,
+               **options) -> torch.Tensor:
+        """``ops.paged_attention`` on a layer's pages (its ``scale``, ``rows``, ``window``, ... as options).
+        ``max_keys``: a bound on the keys that any of the tokens sees, such as the longest row's length;
+        later pages are not looked at, and short rows take a faster form."""
+        table = self.page_table
+        if max_keys is not None:
+            if max_keys <= 0:
+                _refuse("PagedKVCache.attend", f"max_keys {max_keys} must be positive")
+            table = table[:, :-(-max_keys // self.k.shape[2])]
+        return ops.paged_attention(q, self.k[layer], self.v[layer], table, positions, out, **self._scales(layer), **options)
 
     def _scales(self, layer: int) -> dict[str, torch.Tensor]:
         return {n: s[layer] for n, s in (("k_scale", self.k_scale), ("v_scale", self.v_scale)) if s is not None}
