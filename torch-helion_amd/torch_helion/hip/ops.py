@@ -281,8 +281,9 @@ def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
 
 
 # --------------------------------------------------- rotary positions, paged cache
-# One token's calls are shorter on the device than a Python call's bookkeeping, so these take
-# each tensor attribute once, format messages only to raise them and fill a descriptor in one go.
+# One token's calls are shorter on the device than a Python call's bookkeeping, so these test all
+# their tensors in one expression, ask the checks below for the fault only when it fails, and fill
+# a descriptor in one go.
 def _refuse(entry: str, message: str) -> None:
     raise abi.HipBackendError(entry, abi.TH_ERR_INVALID, message)
 
@@ -319,6 +320,11 @@ def _rows_of(t: torch.Tensor, n: int, width: int, dtype: torch.dtype, dev: int, 
         _refuse(entry, f"{name} must be a row-major [{n}, {width}] {dtype} tensor on {_place(dev)}, got {tuple(t.shape)} strides "
                        f"{strides} {t.dtype} on {t.device}")
     return t.data_ptr(), strides[0] if n > 1 else width
+
+
+def _ld(strides: tuple, shape: tuple) -> int:
+    """Row stride of a row-major tensor (a single row's is free, so its width)."""
+    return strides[0] if shape[0] > 1 else shape[1]
 
 
 def _heads(t: torch.Tensor, head_dim: int, entry: str, name: str) -> tuple[int, int]:
@@ -374,16 +380,20 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, out: tor
     output with the same scale it gives the gradient of x. ``out`` may be x; otherwise the two must
     not overlap."""
     entry = "th_rope"
-    n, width = _heads(x, head_dim, entry, "x")
-    dev, dt = x.get_device(), x.dtype
-    if positions.dtype not in (torch.int32, torch.int64):
-        _refuse(entry, f"positions are int32 or int64, got {positions.dtype}")
-    half = freqs.numel()
-    xp, ldx = _rows_of(x, n, width, dt, dev, entry, "x")
-    op, ldo = _rows_of(out, n, width, dt, dev, entry, "out")
-    d = abi.RopeDesc(n, width // head_dim, head_dim, 2 * half, interleaved, inverse, th_dtype(dt), _DT[positions.dtype], scale,
-                     xp, ldx, _vector(positions, n, positions.dtype, dev, entry, "positions"),
-                     _vector(freqs, half, torch.float64, dev, entry, "freqs"), op, ldo)
+    shape = n, width = _heads(x, head_dim, entry, "x")
+    dev, dt, pt, half = x.get_device(), x.dtype, positions.dtype, freqs.numel()
+    sx, so = x.stride(), out.stride()
+    if pt is not torch.int32 and pt is not torch.int64:
+        _refuse(entry, f"positions are int32 or int64, got {pt}")
+    if not (sx[1] == 1 and out.shape == shape and out.dtype is dt and so[1] == 1 and out.get_device() == dev
+            and positions.numel() == n and positions.get_device() == dev and positions.is_contiguous()
+            and freqs.dtype is torch.float64 and freqs.get_device() == dev and freqs.is_contiguous()):
+        _rows_of(x, n, width, dt, dev, entry, "x")
+        _rows_of(out, n, width, dt, dev, entry, "out")
+        _vector(positions, n, pt, dev, entry, "positions")
+        _vector(freqs, half, torch.float64, dev, entry, "freqs")
+    d = abi.RopeDesc(n, width // head_dim, head_dim, 2 * half, interleaved, inverse, th_dtype(dt), _DT[pt], scale,
+                     x.data_ptr(), _ld(sx, shape), positions.data_ptr(), freqs.data_ptr(), out.data_ptr(), _ld(so, shape))
     _launch(entry, d, dev, kernel)
     return out
 
@@ -400,13 +410,18 @@ def _cache(k_cache: torch.Tensor, v_cache: torch.Tensor, dev: int, entry: str) -
     return shape, ks, vs
 
 
-def _table(page_table: torch.Tensor, dev: int, entry: str) -> tuple[int, int, int, int]:
-    """(rows, pages per row, pointer, row stride) of a page table on device ``dev``."""
+def _places(page_table: torch.Tensor, positions: torch.Tensor, rows: torch.Tensor | None, n: int, dev: int, entry: str) -> tuple:
+    """(rows of the table, pages per row, pointer of positions, of rows, of the table, its row stride)."""
     shape, strides = page_table.shape, page_table.stride()
-    if len(shape) != 2 or page_table.dtype is not torch.int32 or (strides[1] != 1 and shape[1] != 1) or page_table.get_device() != dev:
-        _refuse(entry, f"page_table must be a row-major int32 [rows, pages per row] tensor on {_place(dev)}")
-    rows, width = shape
-    return rows, width, page_table.data_ptr(), strides[0] if rows > 1 else width
+    if not (len(shape) == 2 and page_table.dtype is torch.int32 and strides[1] == 1 and page_table.get_device() == dev
+            and positions.dtype is torch.int32 and positions.numel() == n and positions.get_device() == dev
+            and positions.is_contiguous()):
+        if len(shape) != 2 or page_table.dtype is not torch.int32:
+            _refuse(entry, "page_table must be int32 [rows, pages per row]")
+        _rows_of(page_table, shape[0], shape[1], torch.int32, dev, entry, "page_table")
+        _vector(positions, n, torch.int32, dev, entry, "positions")
+    return (shape[0], shape[1], positions.data_ptr(), None if rows is None else _vector(rows, n, torch.int32, dev, entry, "rows"),
+            page_table.data_ptr(), _ld(strides, shape))
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -425,13 +440,14 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, k_ca
     outside the table or the cache is left out and counted in ``n_invalid`` (an int32 device
     scalar that the caller zeroes). Two tokens of a call must not share a slot."""
     entry = "th_paged_append"
-    n, dev, dt = k.shape[0], k.get_device(), k.dtype
+    dev, dt = k.get_device(), k.dtype
     (pages, page_size, hk, hd), ks, vs = _cache(k_cache, v_cache, dev, entry)
-    n_rows, row_pages, tp, ldt = _table(page_table, dev, entry)
-    pos = _vector(positions, n, torch.int32, dev, entry, "positions")
-    rp = None if rows is None else _vector(rows, n, torch.int32, dev, entry, "rows")
-    kp, ldk = _rows_of(k, n, hk * hd, dt, dev, entry, "k")
-    vp, ldv = _rows_of(v, n, hk * hd, dt, dev, entry, "v")
+    shape = n, width = k.shape[0], hk * hd
+    n_rows, row_pages, pos, rp, tp, ldt = _places(page_table, positions, rows, n, dev, entry)
+    sk, sv = k.stride(), v.stride()
+    if not (k.shape == shape and v.shape == shape and v.dtype is dt and sk[1] == 1 and sv[1] == 1 and v.get_device() == dev):
+        _rows_of(k, n, width, dt, dev, entry, "k")
+        _rows_of(v, n, width, dt, dev, entry, "v")
     half, fp = 0, None
     if freqs is not None:
         half = freqs.numel()
@@ -440,15 +456,18 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, k_ca
     if q is not None:
         if q_out is None:
             _refuse(entry, "q needs a q_out")
-        _, width = _heads(q, hd, entry, "q")
-        hq = width // hd
-        qp, ldq = _rows_of(q, n, width, dt, dev, entry, "q")
-        op, ldo = _rows_of(q_out, n, width, torch.bfloat16, dev, entry, "q_out")
+        sq, so, shape_q = q.stride(), q_out.stride(), _heads(q, hd, entry, "q")
+        if not (shape_q[0] == n and q.dtype is dt and sq[1] == 1 and q.get_device() == dev and q_out.shape == shape_q
+                and q_out.dtype is torch.bfloat16 and so[1] == 1 and q_out.get_device() == dev):
+            _rows_of(q, n, shape_q[1], dt, dev, entry, "q")
+            _rows_of(q_out, n, shape_q[1], torch.bfloat16, dev, entry, "q_out")
+        hq, qp, ldq, op, ldo = shape_q[1] // hd, q.data_ptr(), _ld(sq, shape_q), q_out.data_ptr(), _ld(so, shape_q)
     d = abi.PagedAppendDesc(
         n, hq, hk, hd, 2 * half, interleaved, th_dtype(dt), th_dtype(k_cache.dtype), page_size, n_rows, row_pages, pages,
-        rope_scale, 0, pos, rp, tp, ldt, fp, qp, ldq, op, ldo, kp, ldk, vp, ldv,
+        rope_scale, 0, pos, rp, tp, ldt, fp, qp, ldq, op, ldo, k.data_ptr(), _ld(sk, shape), v.data_ptr(), _ld(sv, shape),
         k_cache.data_ptr(), ks[0], ks[1], ks[2], v_cache.data_ptr(), vs[0], vs[1], vs[2],
-        None if k_scale is None else _vector(k_scale, hk, torch.float32, dev, entry, "k_scale"), None if v_scale is None else _vector(v_scale, hk, torch.float32, dev, entry, "v_scale"),
+        None if k_scale is None else _vector(k_scale, hk, torch.float32, dev, entry, "k_scale"),
+        None if v_scale is None else _vector(v_scale, hk, torch.float32, dev, entry, "v_scale"),
         None if n_invalid is None else _vector(n_invalid, 1, torch.int32, dev, entry, "n_invalid"))
     _launch(entry, d, dev, kernel)
 
@@ -487,14 +506,14 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     entry = "th_paged_attention"
     dev = q.get_device()
     (pages, page_size, hk, hd), ks, vs = _cache(k_cache, v_cache, dev, entry)
-    n, width = _heads(q, hd, entry, "q")
-    n_rows, row_pages, tp, ldt = _table(page_table, dev, entry)
-    pos = _vector(positions, n, torch.int32, dev, entry, "positions")
-    rp = None if rows is None else _vector(rows, n, torch.int32, dev, entry, "rows")
+    shape = n, width = _heads(q, hd, entry, "q")
     hq = width // hd
-    qp, ldq = _rows_of(q, n, width, torch.bfloat16, dev, entry, "q")
-    op, ldo = _rows_of(out, n, width, torch.bfloat16, dev, entry, "out")
-    sp = None if slopes is None else _vector(slopes, hq, torch.float32, dev, entry, "slopes")
+    n_rows, row_pages, pos, rp, tp, ldt = _places(page_table, positions, rows, n, dev, entry)
+    sq, so = q.stride(), out.stride()
+    if not (q.dtype is torch.bfloat16 and sq[1] == 1 and out.shape == shape and out.dtype is torch.bfloat16 and so[1] == 1
+            and out.get_device() == dev):
+        _rows_of(q, n, width, torch.bfloat16, dev, entry, "q")
+        _rows_of(out, n, width, torch.bfloat16, dev, entry, "out")
     wp, wn = None, 0
     if workspace is not None:
         if workspace.get_device() != dev or not workspace.is_contiguous():
@@ -507,8 +526,10 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             wp = workspace.data_ptr()
     d = abi.PagedAttnDesc(
         n, hq, hk, hd, th_dtype(k_cache.dtype), page_size, n_rows, row_pages, pages, window, scale, softcap, 0, pos, rp, tp, ldt,
-        qp, ldq, k_cache.data_ptr(), ks[0], ks[1], ks[2], v_cache.data_ptr(), vs[0], vs[1], vs[2],
-        sp, None if k_scale is None else _vector(k_scale, hk, torch.float32, dev, entry, "k_scale"), None if v_scale is None else _vector(v_scale, hk, torch.float32, dev, entry, "v_scale"), op, ldo, wp, wn)
+        q.data_ptr(), _ld(sq, shape), k_cache.data_ptr(), ks[0], ks[1], ks[2], v_cache.data_ptr(), vs[0], vs[1], vs[2],
+        None if slopes is None else _vector(slopes, hq, torch.float32, dev, entry, "slopes"),
+        None if k_scale is None else _vector(k_scale, hk, torch.float32, dev, entry, "k_scale"),
+        None if v_scale is None else _vector(v_scale, hk, torch.float32, dev, entry, "v_scale"), out.data_ptr(), _ld(so, shape), wp, wn)
     _launch(entry, d, dev, kernel)
     return out
 
@@ -543,7 +564,10 @@ def copy_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, src: torch.Tensor, 
     if page_table is not None:
         if page_map is None:
             _refuse(entry, "renaming a page_table needs a page_map")
-        rows, width, tp, ldt = _table(page_table, dev, entry)
+        if page_table.dtype is not torch.int32 or page_table.dim() != 2:
+            _refuse(entry, "page_table must be int32 [rows, pages per row]")
+        rows, width = page_table.shape
+        tp, ldt = _rows_of(page_table, rows, width, torch.int32, dev, entry, "page_table")
         table = (tp, ldt, rows, width, _vector(page_map, pages, torch.int32, dev, entry, "page_map"))
     d = abi.PageCopyDesc(shape[0] if layered else 1, n, pages, page, *operands,
                          _vector(src, n, torch.int32, dev, entry, "src"), _vector(dst, n, torch.int32, dev, entry, "dst"), *table)
