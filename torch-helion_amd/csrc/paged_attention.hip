@@ -537,18 +537,20 @@ __global__ void __launch_bounds__(64 * NW, 8 / NW) paged_attn_kernel(PAttnK p) {
 // Joins the parts of hw heads of one (token, kv head) pair: o = sum_i o_i
 // 2^(m_i - m) / sum_i l_i 2^(m_i - m). Tokens without keys get zeros; pairs that
 // one wave finished are left alone.
-template <int D>
+// A workgroup takes DS of the dims: rows in 256 / (DS / 4) slices.
+template <int D, int DS>
 __global__ void __launch_bounds__(256) paged_attn_join_kernel(PAttnK p, int waves, int hw) {
-  constexpr int LPR = D / 4, NG = 256 / LPR;  // lanes per row, rows at a time
+  constexpr int LPR = DS / 4, NG = 256 / LPR;  // lanes per row, rows at a time
   __shared__ f32x4_t os[NG][LPR];
   __shared__ float ms[NG], ls[NG];
   const int HB = p.Hkv * p.nqb, per = (p.gq + hw - 1) / hw;  // workgroups per pair
-  const int hb = blockIdx.x / per, c0 = (blockIdx.x - hb * per) * hw, t = blockIdx.y, tid = threadIdx.x;
+  const int d0 = blockIdx.x % (D / DS) * DS, bx = blockIdx.x / (D / DS);
+  const int hb = bx / per, c0 = (bx - hb * per) * hw, t = blockIdx.y, tid = threadIdx.x;
   const int kvh = hb / p.nqb, qb = hb - kvh * p.nqb, gn = min(p.gq, p.G - qb * 16);
   const int64_t a = p.prefix[t], tiles = p.prefix[t + 1] - a, all = p.prefix[p.tokens];
   uint16_t* o = p.o + (int64_t)t * p.ldo + (int64_t)(kvh * p.G + qb * 16) * D;
   if (tiles == 0) {
-    for (int e = c0 * D + tid; e < min(gn, c0 + hw) * D; e += 256) o[e] = 0;
+    for (int e = tid; e < (min(gn, c0 + hw) - c0) * DS; e += 256) o[(c0 + e / DS) * D + d0 + e % DS] = 0;
     return;
   }
   const Share share(all, waves / HB);
@@ -573,7 +575,16 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(PAttnK p, int wave
 #pragma unroll 8
     for (int i = slice; i < n; i += slices) {
       const int64_t s = (int64_t)(2 * ((g0 + i) * HB + hb) + (i == 0 && late)) * p.gq + c;
-      add(p.ml[2 * s], p.ml[2 * s + 1], *(const f32x4_t*)(p.part + s * D + 4 * ln));
+      add(p.ml[2 * s], p.ml[2 * s + 1], *(const f32x4_t*)(p.part + s * D + d0 + 4 * ln));
+    }
+  }
+  if (hw == 1) {  // every row is a slice of one head: those of a wave by shuffles
+#pragma unroll
+    for (int d = LPR; d < 64; d <<= 1) {
+      f32x4_t y;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) y[r] = __shfl_xor(x[r], d);
+      add(__shfl_xor(m, d), __shfl_xor(l, d), y);
     }
   }
   os[grp][ln] = x;
@@ -583,10 +594,11 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(PAttnK p, int wave
   }
   __syncthreads();
   if (slice != 0 || c >= gn) return;
-  for (int i = 1; i < slices; ++i) add(ms[i * hw + grp], ls[i * hw + grp], os[i * hw + grp][ln]);
+  const int next = hw == 1 ? 64 / LPR : hw;  // rows apart: one a wave, or one a slice
+  for (int i = next; i + grp < (hw == 1 ? NG : slices * hw); i += next) add(ms[i + grp], ls[i + grp], os[i + grp][ln]);
   const float f = l == 0.f ? 0.f : vscale / l;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) o[c * D + 4 * ln + r] = f32_to_bf16(x[r] * f);
+  for (int r = 0; r < 4; ++r) o[c * D + d0 + 4 * ln + r] = f32_to_bf16(x[r] * f);
 }
 
 template <int D, bool E4>
@@ -722,11 +734,19 @@ extern "C" int th_paged_attention(const th_paged_attn_desc* d, void* stream) {
   }
   launch_paged(k, d->head_dim, e4, false, kLineWaves, (unsigned)grid, s);
   TH_CHECK_LAUNCH();
-  // few pairs: a workgroup for each head, so that their many parts are read at once
-  const int hw = pairs >= 256 ? std::min(k.gq, 1024 / d->head_dim) : 1;
-  const dim3 join((unsigned)(d->heads_kv * k.nqb * cdiv(k.gq, hw)), (unsigned)d->tokens);
-  if (d->head_dim == 128) hipLaunchKernelGGL(paged_attn_join_kernel<128>, join, dim3(256), 0, s, k, waves, hw);
-  else hipLaunchKernelGGL(paged_attn_join_kernel<64>, join, dim3(256), 0, s, k, waves, hw);
+  // Few pairs can be cut into many parts: a workgroup for each head, and for very
+  // few one for each 32 dims of it, reads more of them at once.
+  const int hw = pairs < 256 ? 1 : std::min(k.gq, 1024 / d->head_dim);
+  const bool few = pairs * k.gq <= 128;
+  const int split = few ? d->head_dim / 32 : 1;
+  const dim3 join((unsigned)(d->heads_kv * k.nqb * cdiv(k.gq, hw) * split), (unsigned)d->tokens);
+  if (d->head_dim == 128) {
+    if (few) hipLaunchKernelGGL((paged_attn_join_kernel<128, 32>), join, dim3(256), 0, s, k, waves, hw);
+    else hipLaunchKernelGGL((paged_attn_join_kernel<128, 128>), join, dim3(256), 0, s, k, waves, hw);
+  } else {
+    if (few) hipLaunchKernelGGL((paged_attn_join_kernel<64, 32>), join, dim3(256), 0, s, k, waves, hw);
+    else hipLaunchKernelGGL((paged_attn_join_kernel<64, 64>), join, dim3(256), 0, s, k, waves, hw);
+  }
   TH_CHECK_LAUNCH();
   return TH_OK;
 }
