@@ -182,55 +182,82 @@ __global__ void __launch_bounds__(64 * NW, 8 / NW) paged_attn_kernel(PAttnK p) {
       return;
     }
   } else {
-    __shared__ int64_t pre[64 * NW + 1];  // tiles before each of 64 NW runs of tokens
-    __shared__ int64_t wsum[NW];
-    const int per = (p.tokens + 64 * NW - 1) / (64 * NW);
-    int64_t n = 0;
-    const int t0 = min(p.tokens, tid * per), t1 = min(p.tokens, t0 + per);
-    for (int i = t0; i < t1; ++i) n += span_of<KU>(p, i).units;
-    int64_t inc = n;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int64_t up = __shfl_up(inc, d);
-      if (lane >= d) inc += up;
-    }
-    if (lane == 63) wsum[wave] = inc;
-    __syncthreads();
-    int64_t before = inc - n;
-    for (int w = 0; w < wave; ++w) before += wsum[w];
-    pre[tid] = before;
-    if (tid == 64 * NW - 1) pre[64 * NW] = before + n;
-    if (blockIdx.x == 0) {  // for the join kernel
-      int64_t at = before;
-      for (int i = t0; i < t1; ++i) {
-        p.prefix[i] = at;
-        at += span_of<KU>(p, i).units;
-      }
-      if (tid == 64 * NW - 1) p.prefix[p.tokens] = before + n;
-    }
-    __syncthreads();
     const int groups = (int)gridDim.x * NW / HB;
-    const Share share(pre[64 * NW], groups);
-    if (share.each) steps = share.each + (share.more != 0);
+    int64_t at;  // tiles before token t
     // no step to keep (a tile a wave at most): neighbours on different CUs, so
     // that few tiles spread out
-    me = steps ? (int)blockIdx.x * NW + wave : wave * (int)gridDim.x + (int)blockIdx.x;
-    const int group = me / HB;
-    hb = me - group * HB;
-    u0 = share.begin(group);
-    u1 = group < groups ? share.begin(group + 1) : u0;
+    auto deal = [&](int64_t total) {
+      const Share share(total, groups);
+      if (share.each) steps = share.each + (share.more != 0);
+      me = steps ? (int)blockIdx.x * NW + wave : wave * (int)gridDim.x + (int)blockIdx.x;
+      const int group = me / HB;
+      hb = me - group * HB;
+      u0 = share.begin(group);
+      u1 = group < groups ? share.begin(group + 1) : u0;
+    };
+    if (p.tokens <= 64) {  // a token a lane: every wave counts for itself
+      const int i = min(lane, p.tokens - 1);
+      const int pos = p.positions[i], row = p.rows ? p.rows[i] : i;
+      const uint32_t n = lane < p.tokens ? span_from<KU>(p, pos, row).units : 0;
+      uint32_t inc = n;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t up = __shfl_up(inc, d);
+        if (lane >= d) inc += up;
+      }
+      const uint32_t total = __builtin_amdgcn_readlane(inc, 63);
+      if (blockIdx.x == 0 && wave == 0) {  // for the join kernel
+        if (lane < p.tokens) p.prefix[lane] = inc - n;
+        if (lane == 0) p.prefix[p.tokens] = total;
+      }
+      deal(total);
+      t = __popcll(__ballot(lane < p.tokens && inc - n <= u0)) - 1;  // the last that begins at or before u0
+      at = (uint32_t)__builtin_amdgcn_readlane(inc - n, t);
+      sp = span_from<KU>(p, __builtin_amdgcn_readlane(pos, t), __builtin_amdgcn_readlane(row, t));
+    } else {
+      __shared__ int64_t pre[64 * NW + 1];  // tiles before each of 64 NW runs of tokens
+      __shared__ int64_t wsum[NW];
+      const int per = (p.tokens + 64 * NW - 1) / (64 * NW);
+      int64_t n = 0;
+      const int t0 = min(p.tokens, tid * per), t1 = min(p.tokens, t0 + per);
+      for (int i = t0; i < t1; ++i) n += span_of<KU>(p, i).units;
+      int64_t inc = n;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int64_t up = __shfl_up(inc, d);
+        if (lane >= d) inc += up;
+      }
+      if (lane == 63) wsum[wave] = inc;
+      __syncthreads();
+      int64_t before = inc - n;
+      for (int w = 0; w < wave; ++w) before += wsum[w];
+      pre[tid] = before;
+      if (tid == 64 * NW - 1) pre[64 * NW] = before + n;
+      if (blockIdx.x == 0) {
+        int64_t sum = before;
+        for (int i = t0; i < t1; ++i) {
+          p.prefix[i] = sum;
+          sum += span_of<KU>(p, i).units;
+        }
+        if (tid == 64 * NW - 1) p.prefix[p.tokens] = before + n;
+      }
+      __syncthreads();
+      deal(pre[64 * NW]);
+      int run = -1;  // the last run that begins at or before u0
+      for (int i = 0; i < NW; ++i) run += __popcll(__ballot(pre[64 * i + lane] <= u0));
+      t = run * per;
+      at = pre[run];
+      if (u0 < u1) {
+        sp = span_of<KU>(p, t);
+        while (at + sp.units <= u0 && t < p.tokens - 1) {
+          at += sp.units;
+          sp = span_of<KU>(p, ++t);
+        }
+      }
+    }
     if (u0 >= u1) {
       for (; step < steps; ++step) barrier_keep_loads();
       return;
-    }
-    int run = -1;  // the last run that begins at or before u0
-    for (int i = 0; i < NW; ++i) run += __popcll(__ballot(pre[64 * i + lane] <= u0));
-    t = run * per;
-    int64_t at = pre[run];
-    sp = span_of<KU>(p, t);
-    while (at + sp.units <= u0 && t < p.tokens - 1) {
-      at += sp.units;
-      sp = span_of<KU>(p, ++t);
     }
     k = (int)(u0 - at);
   }
