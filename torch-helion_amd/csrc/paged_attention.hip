@@ -437,10 +437,11 @@ __global__ void __launch_bounds__(64 * NW, 8 / NW) paged_attn_kernel(PAttnK p) {
           s[b][r] = x;
         }
       if (p.slopes) {  // from the last key: what lies between it and pos is the same for all
+        const float far = slope * (float)(cs.hi - 1 - j0 - 4 * g);
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) s[b][r] -= slope * (float)(cs.hi - 1 - (j0 + 16 * b + 4 * g + r));
+          for (int r = 0; r < 4; ++r) s[b][r] = fmaf(slope, (float)(16 * b + r), s[b][r] - far);
       }
       if (j0 < cs.lo || j0 + KT > cs.hi || ok != (1u << NB) - 1) {
 #pragma unroll
