@@ -368,16 +368,17 @@ int th_paged_append(const th_paged_append_desc* desc, void* stream);
  * key (padded, or of a row outside the table) gets zeros. What the slots of
  * unseen keys hold, NaN included, does not reach the result. The keys of all
  * tokens are dealt out evenly over the GPU, whatever the lengths, and the
- * parts are joined through the workspace (which short rows do not need).
+ * parts are joined through the workspace (which short rows do not need). o may
+ * be q (same row stride).
  */
 typedef struct th_paged_attn_desc {
-  int32_t tokens, heads_q, heads_kv, head_dim;  /* head_dim 64 or 128 */
+  int32_t tokens, heads_q, heads_kv, head_dim;  /* tokens <= 65535, head_dim 64 or 128 */
   int32_t cache_dtype;                  /* TH_BF16 or TH_F8E4M3; q and o are bf16 */
   int32_t page_size;                    /* a power of two, at least 16 */
   int32_t n_rows, row_pages;
   int64_t pages;
   int32_t window;                       /* 0: none */
-  float scale, softcap;                 /* softcap 0: none */
+  float scale, softcap;                 /* softcap 0: none; at most 1024 */
   int32_t pad_;
   const int32_t* positions;             /* [tokens] */
   const int32_t* rows;                  /* optional [tokens] */

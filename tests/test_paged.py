@@ -126,7 +126,7 @@ REFUSED = [
     ("th_paged_attention", attn_desc, [
         ({"heads_q": 5}, "multiple"), ({"head_dim": 96}, "head_dim"), ({"cache_dtype": 0}, "cache_dtype"), ({"page_size": 8}, "page_size"),
         ({"page_size": 48}, "page_size"), ({"row_pages": 0}, "page table"), ({"window": -1}, "window"), ({"softcap": -1.0}, "softcap"),
-        ({"softcap": float("nan")}, "softcap"), ({"ld_q": 255}, "row strides"), ({"ld_q": 260}, "16 bytes"),
+        ({"softcap": float("nan")}, "softcap"), ({"softcap": 1025.0}, "softcap"), ({"tokens": 65536}, "tokens"), ({"ld_q": 255}, "row strides"), ({"ld_q": 260}, "16 bytes"),
         ({"k_stride_h": 68}, "16 bytes"), ({"v_stride_page": 2050}, "16 bytes"), ({"cache_dtype": 3, "k_stride_t": 136}, "16 bytes"),
         ({"k_stride_t": 1 << 23}, "token strides"), ({"q": 16392}, "16-byte"), ({"v_cache": 65544}, "16-byte"), ({"v_scale": 4096}, "e4m3"),
         ({"tokens": -1}, "tokens"), ({"tokens": 5}, "exceed the table"), ({"positions": 0}, "null"), ({"o": 0}, "null"),

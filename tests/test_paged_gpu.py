@@ -379,6 +379,35 @@ def test_attention_rows_and_head_major_pages(gpu):
     check_attention(gpu, [40, 41, 900], 4, 4, 64, 16, rows=[1, 1, 0], head_major=True, cache=E4M3)
 
 
+def test_attention_cap_far_above_the_scores(gpu):
+    """The largest cap leaves scores of a few units nearly as they are; the bound's 2^-20 softcap is then 1e-3."""
+    from torch_helion.hip import ops
+
+    announce("paged attention, a cap far above the scores")
+    kc, vc, table = paged(2, 40, 16, 2, 64, BF16, gen(12), gpu)
+    q = (torch.randn(2, 4 * 64, generator=gen(13)) * 2).to(BF16)
+    pos = torch.tensor([630, 99], dtype=torch.int32)
+    out = torch.empty_like(q, device=gpu)
+    ops.paged_attention(q.to(gpu), kc, vc, table, pos.to(gpu), out, scale=0.125, softcap=1024.0)
+    ref, mag, err = attention64(q.view(2, 4, 64), kc.float().cpu(), vc.float().cpu(), table.cpu(), pos, None, 0.125, softcap=1024.0)
+    assert_within(out.view(2, 4, 64), ref, u(BF16) * (ref.abs() + mag) * (1 + 2 * u(BF16)) + 2 * err * mag)
+
+
+@pytest.mark.parametrize("row_pages", [20, 200])
+def test_attention_onto_its_queries(gpu, row_pages):
+    """out may be q, in both forms."""
+    from torch_helion.hip import ops
+
+    announce(f"paged attention onto its queries, rows of {row_pages} pages")
+    kc, vc, table = paged(9, row_pages, 16, 4, 64, BF16, gen(14), gpu)
+    q = torch.randn(9, 12 * 64, generator=gen(15)).to(BF16).to(gpu)
+    pos = torch.tensor([0, 319, 5, -1, 100, 250, 16, 31, 200], dtype=torch.int32, device=gpu)
+    out = torch.empty_like(q)
+    ops.paged_attention(q, kc, vc, table, pos, out, scale=0.125)
+    ops.paged_attention(q, kc, vc, table, pos, q, scale=0.125)
+    assert torch.equal(q, out)
+
+
 def test_attention_outside_the_table(gpu):
     """A position past the table sees the table's keys; a row outside it sees none; pages outside the cache
     are left out, also where that leaves nothing."""

@@ -695,7 +695,10 @@ extern "C" int th_paged_attention(const th_paged_attn_desc* d, void* stream) {
   TH_CHECK_ARG(d->n_rows > 0 && d->row_pages > 0 && d->pages > 0 && d->ld_page_table >= d->row_pages,
                "th_paged_attention: bad page table sizes");
   TH_CHECK_ARG((int64_t)d->row_pages * d->page_size < (int64_t)1 << 30, "th_paged_attention: row of 2^30 keys or more");
-  TH_CHECK_ARG(d->window >= 0 && d->softcap >= 0.f, "th_paged_attention: window and softcap must not be negative");
+  // The capped score's error is 1e-7 of the cap (its tanh is 1 - 2 / (1 + e^2x)): up
+  // to here 1e-4, a fortieth of what rounding p to bf16 does.
+  TH_CHECK_ARG(d->window >= 0 && d->softcap >= 0.f && d->softcap <= 1024.f,
+               "th_paged_attention: window %d must not be negative, softcap %g in 0..1024", d->window, (double)d->softcap);
   const int64_t row = (int64_t)d->heads_q * d->head_dim;
   TH_CHECK_ARG(d->ld_q >= row && d->ld_o >= row, "th_paged_attention: q/o row strides smaller than heads_q*head_dim");
   const int per = d->cache_dtype == TH_BF16 ? 8 : 16;  // elements in 16 bytes

@@ -496,13 +496,15 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
                     workspace: torch.Tensor | None = None, kernel: str | None = None) -> torch.Tensor:
     """One query per token against the pages of its row (see :func:`paged_append` for the caches,
-    ``positions`` and ``rows``). ``q``/``out``: [tokens, heads_q * head_dim] bf16.
+    ``positions`` and ``rows``). ``q``/``out``: [tokens, heads_q * head_dim] bf16, at most 65535
+    tokens; ``out`` may be ``q``. head_dim is 64 or 128, the pages hold 16 tokens or more.
 
     The token at position p sees the keys 0 .. p of its row, the last ``window`` of them if given.
-    Scores are ``scale q . k``, capped as ``softcap tanh(s / softcap)`` if given, then biased by
+    Scores are ``scale q . k``, capped as ``softcap tanh(s / softcap)`` if given (at most 1024), then biased by
     ``-slopes[h] (p - j)`` (fp32 [heads_q]) if given. A token without keys gets zeros.
     ``workspace``: :func:`paged_attention_workspace_bytes` bytes that no concurrent call uses;
-    without one the call takes it from torch's allocator."""
+    without one the call takes it from torch's allocator. A table cut to the pages in use
+    (``page_table[:, :n]``) lets short rows take a faster form."""
     entry = "th_paged_attention"
     dev = q.get_device()
     (pages, page_size, hk, hd), ks, vs = _cache(k_cache, v_cache, dev, entry)
