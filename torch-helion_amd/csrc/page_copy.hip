@@ -3,7 +3,11 @@
 // counterpart in the reference, which has no cache).
 //
 // HBM bound: each byte is read once and written once. One workgroup moves one
-// 16 KiB piece of one page of one tensor of one layer.
+// 32 KiB piece of one page of one tensor of one layer: eight 16-byte loads a
+// lane, then the stores, both past the caches (nothing is used twice). 683 pages
+// of 64 KiB in 8 layers of both caches, 1.43 GB: 266 us, 5.39 TB/s (282 us with
+// 16 KiB pieces through the caches, 277 with the stores alone past them; a large
+// device copy reaches 4.95 TB/s).
 #include "common.h"
 
 namespace th {
@@ -19,7 +23,7 @@ struct PageCopyK {
   int n, layers, pieces, row_pages, copy_blocks;
 };
 
-constexpr int kPiece = 16384;
+constexpr int kPiece = 32768;
 
 __global__ void __launch_bounds__(256) page_copy_kernel(PageCopyK p) {
   int64_t b = blockIdx.x;
@@ -43,7 +47,18 @@ __global__ void __launch_bounds__(256) page_copy_kernel(PageCopyK p) {
   const char* from = base + src * stride;
   char* to = base + dst * stride;
   const int n = (int)min((int64_t)kPiece, p.bytes - (int64_t)piece * kPiece);
-  for (int o = threadIdx.x * 16; o < n; o += 256 * 16) *(uint4*)(to + o) = *(const uint4*)(from + o);
+  // buffer accesses: past n bytes a load is zero and a store is dropped
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  constexpr int kNt = 2;  // cache policy: non-temporal
+  const auto rf = __builtin_amdgcn_make_buffer_rsrc((void*)from, 0, n, 0x00020000);
+  const auto rt = __builtin_amdgcn_make_buffer_rsrc((void*)to, 0, n, 0x00020000);
+  u32x4 x[kPiece / 4096];
+#pragma unroll
+  for (int i = 0; i < kPiece / 4096; ++i)
+    x[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rf, threadIdx.x * 16 + i * 4096, 0, kNt));
+#pragma unroll
+  for (int i = 0; i < kPiece / 4096; ++i)
+    __builtin_amdgcn_raw_buffer_store_b128(x[i], rt, threadIdx.x * 16 + i * 4096, 0, kNt);
 }
 
 }  // namespace th
