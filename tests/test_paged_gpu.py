@@ -257,6 +257,34 @@ def test_append_leaves_out_what_lies_outside(gpu):
     assert (q_out[6] == 0).all()
 
 
+@pytest.mark.parametrize("dtype,cache", [(BF16, E4M3), (torch.float32, BF16)])
+def test_large_calls_equal_their_halves(gpu, dtype, cache):
+    """Calls past 128 MB go past the caches: the same bits as two calls of half the tokens each, which do not."""
+    from torch_helion.hip import ops
+
+    announce(f"large rope and append {dtype} -> {cache}")
+    t, hq, hk, d, ps = 6000 if dtype == torch.float32 else 9000, 24, 8, 128, 64
+    g = torch.Generator(device=gpu).manual_seed(4)
+    qkv = torch.randn(t, (hq + 2 * hk) * d, generator=g, device=gpu).to(dtype)
+    q, k, v = qkv.split([hq * d, hk * d, hk * d], 1)
+    f = ops.rope_frequencies(96, 10000.0, device=gpu)
+    pos, rows = torch.arange(t, dtype=torch.int32, device=gpu), torch.zeros(t, dtype=torch.int32, device=gpu)
+    pages = -(-t // ps)
+    table = torch.randperm(pages, generator=g, device=gpu).view(1, pages).to(torch.int32)
+    results = []
+    for parts in (1, 2):
+        caches = [torch.zeros(pages, ps, hk, d, device=gpu).to(cache) for _ in range(2)]
+        q_out = torch.zeros(t, hq * d, dtype=BF16, device=gpu)
+        turned = torch.zeros_like(qkv)
+        for s in torch.arange(t, device=gpu).tensor_split(parts):
+            a, b = int(s[0]), int(s[-1]) + 1
+            ops.paged_append(k[a:b], v[a:b], pos[a:b], *caches, table, rows=rows[a:b], freqs=f, q=q[a:b], q_out=q_out[a:b])
+            ops.rope(qkv[a:b], pos[a:b], f, turned[a:b], head_dim=d)
+        results.append((*caches, q_out, turned))
+    for a, b in zip(*results):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 def test_append_special_values(gpu):
     """An e4m3 cache saturates, infinities too, and keeps NaN."""
     from torch_helion.hip import ops
