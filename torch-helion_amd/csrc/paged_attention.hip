@@ -149,8 +149,13 @@ struct PaTile {
 
 constexpr int kLineWaves = 8;
 
-// NW: waves of a workgroup.
-template <int D, bool E4, bool PAIR, int NW>
+// NW: waves of a workgroup. NT: V is loaded past the caches (non-temporal), which
+// leaves them to K, whose loads take half a 128-byte line each. In a graph, with
+// and without: 64 sequences of 2048-4096 keys 140.6 / 149.8 us, with an 8-bit cache
+// 100.4 / 106.7, two of 100-131k 165 / 177; K past the caches too 147, 107, 175.
+// Where everything a loop reads stays in the 256 MB last-level cache it costs: 256
+// pairs of 256-512 keys (50 MB) 14.3 / 13.8, 512 pairs of 512-1024 (200 MB) 36.5 / 42.7.
+template <int D, bool E4, bool PAIR, int NW, bool NT>
 __global__ void __launch_bounds__(64 * NW, 8 / NW) paged_attn_kernel(PAttnK p) {
   using T = PaTile<D, E4>;
   constexpr int KU = PAIR ? NW * T::KT : T::KT;  // keys of a step: of the workgroup's, or of one wave's
@@ -328,7 +333,7 @@ __global__ void __launch_bounds__(64 * NW, 8 / NW) paged_attn_kernel(PAttnK p) {
       for (int i = 0; i < 16 / RPI; ++i) {
         const int r = i * RPI + lr;
         const int off = jb + r >= sp.lo ? r * (int)p.vt + 16 * lc : 0x7ffffff0;
-        vr[b * (16 / RPI) + i] = __builtin_bit_cast(pa_u32x4, __builtin_amdgcn_raw_buffer_load_b128(vres, off, 0, 0));
+        vr[b * (16 / RPI) + i] = __builtin_bit_cast(pa_u32x4, __builtin_amdgcn_raw_buffer_load_b128(vres, off, 0, NT ? 2 : 0));
       }
     }
   };
@@ -629,21 +634,24 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(PAttnK p, int wave
   for (int r = 0; r < 4; ++r) o[c * D + d0 + 4 * ln + r] = f32_to_bf16(x[r] * f);
 }
 
+enum PagedForm { kLine, kPair8, kPair4, kPair4Nt };
+
 template <int D, bool E4>
-static void launch_paged_as(const PAttnK& k, bool pair, int waves, unsigned grid, hipStream_t s) {
-  const dim3 g(grid), b(64 * waves);
-  if (!pair) hipLaunchKernelGGL((paged_attn_kernel<D, E4, false, kLineWaves>), g, b, 0, s, k);
-  else if (waves == 8) hipLaunchKernelGGL((paged_attn_kernel<D, E4, true, 8>), g, b, 0, s, k);
-  else hipLaunchKernelGGL((paged_attn_kernel<D, E4, true, 4>), g, b, 0, s, k);
+static void launch_paged_as(const PAttnK& k, PagedForm form, unsigned grid, hipStream_t s) {
+  const dim3 g(grid);
+  if (form == kLine) hipLaunchKernelGGL((paged_attn_kernel<D, E4, false, kLineWaves, true>), g, dim3(64 * kLineWaves), 0, s, k);
+  else if (form == kPair8) hipLaunchKernelGGL((paged_attn_kernel<D, E4, true, 8, false>), g, dim3(512), 0, s, k);
+  else if (form == kPair4) hipLaunchKernelGGL((paged_attn_kernel<D, E4, true, 4, false>), g, dim3(256), 0, s, k);
+  else hipLaunchKernelGGL((paged_attn_kernel<D, E4, true, 4, true>), g, dim3(256), 0, s, k);
 }
 
-static void launch_paged(const PAttnK& k, int head_dim, bool e4, bool pair, int waves, unsigned grid, hipStream_t s) {
+static void launch_paged(const PAttnK& k, int head_dim, bool e4, PagedForm form, unsigned grid, hipStream_t s) {
   if (head_dim == 128) {
-    if (e4) launch_paged_as<128, true>(k, pair, waves, grid, s);
-    else launch_paged_as<128, false>(k, pair, waves, grid, s);
+    if (e4) launch_paged_as<128, true>(k, form, grid, s);
+    else launch_paged_as<128, false>(k, form, grid, s);
   } else {
-    if (e4) launch_paged_as<64, true>(k, pair, waves, grid, s);
-    else launch_paged_as<64, false>(k, pair, waves, grid, s);
+    if (e4) launch_paged_as<64, true>(k, form, grid, s);
+    else launch_paged_as<64, false>(k, form, grid, s);
   }
 }
 
@@ -759,11 +767,12 @@ extern "C" int th_paged_attention(const th_paged_attn_desc* d, void* stream) {
     // eight waves where there is a CU for each pair and they have more than a tile
     // each (256 pairs, 16 tiles of e4m3: 16.1 us against 16.7, 32 tiles 24.1 against
     // 27.5), else four (4 tiles 6.2 against 7.0; 512 pairs would wait for CUs)
-    launch_paged(k, d->head_dim, e4, true, pairs <= device_cus() && tiles > 8 ? 8 : 4, (unsigned)pairs, s);
+    const PagedForm form = pairs <= device_cus() && tiles > 8 ? kPair8 : pairs * tiles > (128 << 20) / 16384 ? kPair4Nt : kPair4;
+    launch_paged(k, d->head_dim, e4, form, (unsigned)pairs, s);
     TH_CHECK_LAUNCH();
     return TH_OK;
   }
-  launch_paged(k, d->head_dim, e4, false, kLineWaves, (unsigned)grid, s);
+  launch_paged(k, d->head_dim, e4, kLine, (unsigned)grid, s);
   TH_CHECK_LAUNCH();
   // Few pairs can be cut into many parts: a workgroup for each head, and for very
   // few one for each 32 dims of it, reads more of them at once.
