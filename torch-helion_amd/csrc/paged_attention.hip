@@ -16,27 +16,29 @@
 //            known on the host (a captured graph serves any lengths). The parts
 //            of a token that was cut go through the workspace (m, l, o in fp32)
 //            to the join kernel; a token inside one stretch is finished by its
-//            group. The waves of a CU keep step with a barrier a tile: left
-//            alone, the older half of them is served first and ends at 108 us
-//            where the younger ends at 134 (64 sequences of 2048-4096 keys); and
-//            the heads of a key, neighbours in memory, are read together.
+//            group. The waves of a CU keep step (keep_step): left alone, the
+//            older half of them is served first and ends at 108 us where the
+//            younger ends at 134 (64 sequences of 2048-4096 keys); and the heads of
+//            a key, neighbours in memory, are read together.
 //   pair     a workgroup for each (token, kv head) pair, its tiles dealt out to
 //            the waves in turn and the waves merged in LDS: where a pair can have
 //            only a few tiles by its table and window, one launch and no line to
 //            lay out.
 //
 // One tile:
-//   K        loaded straight in the operand layout of S^T = K Q^T
-//            (v_mfma_f32_16x16x32_bf16: lane l holds row l % 16 and 8 dims from
-//            8 (l / 16)): 16 bytes a lane, 64 contiguous bytes a row. The dims of
-//            an e4m3 row are permuted (16 consecutive ones serve two k steps,
-//            q alike), so that those loads are 16 bytes too.
-//   V        loaded by rows, written to the wave's own LDS slice as bf16, and
-//            read transposed (ds_read_b64_tr_b16) for O^T += V^T P^T; P^T is the
-//            S^T accumulators as they are, rounded to bf16 (half a step is 2^-8 of
-//            each p; sums and maxima stay fp32).
-// The next tile's loads are issued as soon as S^T has used K, and land during
-// the softmax and the second product. Buffer loads return zero past their
+//   V        loaded by whole rows (16-byte pieces, consecutive lanes next to each
+//            other) and staged as bf16 in the wave's own LDS slice, swizzled.
+//   S^T      = K Q^T, v_mfma_f32_16x16x32_bf16: lane l supplies row l % 16 and 8
+//            dims from 8 (l / 16). A bf16 K goes through the slice too, before V:
+//            loaded in its operand layout, half a 128-byte line of 16 rows at a
+//            time, 64 sequences of 2048-4096 keys took 139.7 us for 134.4. An e4m3
+//            K is loaded in that layout, the dims of a row permuted (16 consecutive
+//            ones serve two k steps, q alike): 100.3 us, through the slice 101.6.
+//   O^T      += V^T P^T: V is read transposed (ds_read_b64_tr_b16); P^T is the S^T
+//            accumulators as they are, rounded to bf16 (half a step is 2^-8 of each
+//            p; sums and maxima stay fp32).
+// The next tile's loads are issued as soon as V is staged, and land during the
+// softmax and the second product. Buffer loads return zero past their
 // range: unseen slots of a page and pages outside the cache cost no branch, and
 // whatever they hold (NaN) never meets a zero probability.
 #include "common.h"
@@ -132,10 +134,18 @@ __device__ __forceinline__ bf16x8_t e4m3x8_to_bf16(unsigned lo, unsigned hi) {
   return u.v;
 }
 
-// LDS slot of 16-byte chunk c of V row r is c ^ sw(r): a transposing read (16
-// rows, 32 bytes each) then hits every bank twice.
+// LDS slot of 16-byte chunk c of K row r is c ^ ksw(r): the 16 rows of an operand
+// read then hit distinct banks.
+template <int CPR>
+__device__ __forceinline__ int pa_ksw(int r) { return CPR == 16 ? r & 15 : CPR == 8 ? (r >> 1) & 7 : (r >> 2) & 3; }
+
+// The same of V as bf16: a transposing read (16 rows, 32 bytes each) hits every
+// bank twice. The lowest bit lets neighbouring rows of e4m3, whose 16-byte pieces
+// become two chunks each, write to even and odd slots at once.
 template <int D>
-__device__ __forceinline__ int pa_sw(int r) { return D == 128 ? 2 * (r & 7) : 2 * ((r >> 1) & 3); }
+__device__ __forceinline__ int pa_sw(int r) {
+  return D == 128 ? 2 * (r & 7) + (r & 1) : 2 * ((r >> 1) & 3) + ((r >> 1) & 1);
+}
 
 template <int D, bool E4>
 struct PaTile {
@@ -144,23 +154,31 @@ struct PaTile {
   static constexpr int NB = KT / 16;            // 16-key blocks
   static constexpr int CPR = RB / 16;           // 16-byte chunks per row
   static constexpr int RPI = 64 / CPR;          // V rows per load instruction
-  static constexpr int LDS = KT * D * 2;        // one wave's V tile, bf16
+  static constexpr int LDS = KT * D * 2;        // one wave's slice: V as bf16, K (as it is) before it
 };
 
 constexpr int kLineWaves = 8;
 
-// NW: waves of a workgroup. NT: V is loaded past the caches (non-temporal), which
-// leaves them to K, whose loads take half a 128-byte line each. In a graph, with
-// and without: 64 sequences of 2048-4096 keys 140.6 / 149.8 us, with an 8-bit cache
-// 100.4 / 106.7, two of 100-131k 165 / 177; K past the caches too 147, 107, 175.
-// Where everything a loop reads stays in the 256 MB last-level cache it costs: 256
-// pairs of 256-512 keys (50 MB) 14.3 / 13.8, 512 pairs of 512-1024 (200 MB) 36.5 / 42.7.
-template <int D, bool E4, bool PAIR, int NW, bool NT>
+// The waves of a line's workgroup meet at every other tile: with a barrier at each
+// one 64 sequences of 2048-4096 keys took 134.4 us for 131.3 (an 8-bit cache 100.5
+// for 96.7), at every fourth 130.6 (99.0).
+__device__ __forceinline__ void keep_step(int64_t step) {
+  if ((step & 1) == 0) barrier_keep_loads();
+}
+
+// NW: waves of a workgroup. NT: what is loaded past the caches (non-temporal): 1 V,
+// 2 a bf16 K too. In a graph, us, with neither, V, both: 64 sequences of 2048-4096
+// keys 149.4, 136.1, 132.1, two of 100-131k 176, 161, 157; an 8-bit cache 105.4
+// without and 97.3 with (its K, in half lines, past the caches too: 107). Where
+// what is read stays in the 256 MB last-level cache it costs: 288 windows of 1000
+// (pair form) 17.0, 19.5, 20.1, 64 short lines (82 MB) 25.2, 26.3, 27.6; caches of
+// that size that are not there yet, 16 sequences of 500-4000 keys: 40.2, 37.2, 37.9.
+template <int D, bool E4, bool PAIR, int NW, int NT>
 __global__ void __launch_bounds__(64 * NW, 8 / NW) paged_attn_kernel(PAttnK p) {
   using T = PaTile<D, E4>;
   constexpr int KU = PAIR ? NW * T::KT : T::KT;  // keys of a step: of the workgroup's, or of one wave's
   constexpr int RB = T::RB, KT = T::KT, NB = T::NB, CPR = T::CPR, RPI = T::RPI;
-  constexpr int NKS = D / 32, NDB = D / 16, JPR = RB / 64;  // JPR: K loads per 16-key block
+  constexpr int NKS = D / 32, NDB = D / 16, JPR = RB / 64;  // JPR: loads per 16-key block
   constexpr int OW = PAIR ? NW * 16 * D * 4 : 0;  // the merge's o rows share the V tiles' LDS
   __shared__ __attribute__((aligned(16))) char smem[NW * T::LDS > OW ? NW * T::LDS : OW];
 
@@ -261,7 +279,7 @@ __global__ void __launch_bounds__(64 * NW, 8 / NW) paged_attn_kernel(PAttnK p) {
       }
     }
     if (u0 >= u1) {
-      for (; step < steps; ++step) barrier_keep_loads();
+      for (; step < steps; ++step) keep_step(step);
       return;
     }
     k = (int)(u0 - at);
@@ -279,7 +297,7 @@ __global__ void __launch_bounds__(64 * NW, 8 / NW) paged_attn_kernel(PAttnK p) {
   const int e4 = (lane & 15) >> 2, j4 = lane & 3;
   const int vr0 = 4 * g + e4;
   const int vxo = pa_sw<D>(vr0) >> 1;
-  const char* rv = sv + vr0 * D * 2 + (j4 >> 1) * 16 + (j4 & 1) * 8;
+  const char* rv = sv + vr0 * D * 2 + ((j4 >> 1) ^ (pa_sw<D>(vr0) & 1)) * 16 + (j4 & 1) * 8;
 
   // ---- the load cursor (t, k; sp): one tile ahead of the computation, also over the
   // ends of tokens
@@ -326,14 +344,13 @@ __global__ void __launch_bounds__(64 * NW, 8 / NW) paged_attn_kernel(PAttnK p) {
       const auto kres = __builtin_amdgcn_make_buffer_rsrc((void*)kpage, 0, ok ? (int)((rows - 1) * p.kt) + RB : 0, 0x00020000);
       const auto vres = __builtin_amdgcn_make_buffer_rsrc((void*)vpage, 0, ok ? (int)((rows - 1) * p.vt) + RB : 0, 0x00020000);
 #pragma unroll
-      for (int j = 0; j < JPR; ++j)
-        kr[b * JPR + j] = __builtin_bit_cast(
-            pa_u32x4, __builtin_amdgcn_raw_buffer_load_b128(kres, qc * (int)p.kt + 64 * j + 16 * g, 0, 0));
-#pragma unroll
-      for (int i = 0; i < 16 / RPI; ++i) {
+      for (int i = 0; i < JPR; ++i) {
         const int r = i * RPI + lr;
         const int off = jb + r >= sp.lo ? r * (int)p.vt + 16 * lc : 0x7ffffff0;
-        vr[b * (16 / RPI) + i] = __builtin_bit_cast(pa_u32x4, __builtin_amdgcn_raw_buffer_load_b128(vres, off, 0, NT ? 2 : 0));
+        const int koff = E4 ? qc * (int)p.kt + 64 * i + 16 * g : r * (int)p.kt + 16 * lc;
+        kr[b * JPR + i] =
+            __builtin_bit_cast(pa_u32x4, __builtin_amdgcn_raw_buffer_load_b128(kres, koff, 0, NT > 1 ? 2 : 0));
+        vr[b * JPR + i] = __builtin_bit_cast(pa_u32x4, __builtin_amdgcn_raw_buffer_load_b128(vres, off, 0, NT ? 2 : 0));
       }
     }
   };
@@ -386,26 +403,39 @@ __global__ void __launch_bounds__(64 * NW, 8 / NW) paged_attn_kernel(PAttnK p) {
       u_begin = u;
     }
     f32x4_t s[NB];
-    if (busy) {
-      pa_lds_order();
+    auto stage_k = [&]() {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = i * RPI + lr;
+        *(pa_u32x4*)(sv + r * RB + ((lc ^ pa_ksw<CPR>(r)) << 4)) = kr[i];
+      }
+    };
+    auto stage_v = [&]() {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int r = i * RPI + lr;
         if constexpr (E4) {
-          char* w = sv + r * D * 2 + (((2 * lc) ^ pa_sw<D>(r)) << 4);
-          *(bf16x8_t*)w = e4m3x8_to_bf16(vr[i][0], vr[i][1]);
-          *(bf16x8_t*)(w + 16) = e4m3x8_to_bf16(vr[i][2], vr[i][3]);
+          const int at_ = ((2 * lc) ^ pa_sw<D>(r)) << 4;
+          *(bf16x8_t*)(sv + r * D * 2 + at_) = e4m3x8_to_bf16(vr[i][0], vr[i][1]);
+          *(bf16x8_t*)(sv + r * D * 2 + (at_ ^ 16)) = e4m3x8_to_bf16(vr[i][2], vr[i][3]);
         } else {
           *(pa_u32x4*)(sv + r * D * 2 + ((lc ^ pa_sw<D>(r)) << 4)) = vr[i];
         }
       }
+    };
+    if (busy) {
+      pa_lds_order();  // the tile before has been read
+      if constexpr (E4) stage_v();
+      else stage_k();
+      pa_lds_order();
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[b][r] = 0.f;
 #pragma unroll
         for (int j = 0; j < JPR; ++j) {
-          const pa_u32x4 x = kr[b * JPR + j];
+          const int row = 16 * b + qc;
+          const pa_u32x4 x = E4 ? kr[b * JPR + j] : *(const pa_u32x4*)(sv + row * RB + (((4 * j + g) ^ pa_ksw<CPR>(row)) << 4));
           if constexpr (E4) {
             s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e4m3x8_to_bf16(x[0], x[1]), qf[2 * j], s[b], 0, 0, 0);
             s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e4m3x8_to_bf16(x[2], x[3]), qf[2 * j + 1], s[b], 0, 0, 0);
@@ -413,6 +443,10 @@ __global__ void __launch_bounds__(64 * NW, 8 / NW) paged_attn_kernel(PAttnK p) {
             s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, x), qf[j], s[b], 0, 0, 0);
           }
         }
+      }
+      if constexpr (!E4) {
+        pa_lds_order();  // a wave's LDS accesses complete in order: V may replace K
+        stage_v();
       }
     }
     ++u;
@@ -496,7 +530,7 @@ __global__ void __launch_bounds__(64 * NW, 8 / NW) paged_attn_kernel(PAttnK p) {
         }
     }
     if (step < steps) {
-      barrier_keep_loads();
+      keep_step(step);
       ++step;
     }
     fresh = ends;
@@ -564,7 +598,7 @@ __global__ void __launch_bounds__(64 * NW, 8 / NW) paged_attn_kernel(PAttnK p) {
     }
     if (!more) break;
   }
-  for (; step < steps; ++step) barrier_keep_loads();
+  for (; step < steps; ++step) keep_step(step);
 }
 
 // Joins the parts of hw heads of one (token, kv head) pair: o = sum_i o_i
@@ -634,15 +668,17 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(PAttnK p, int wave
   for (int r = 0; r < 4; ++r) o[c * D + d0 + 4 * ln + r] = f32_to_bf16(x[r] * f);
 }
 
-enum PagedForm { kLine, kPair8, kPair4, kPair4Nt };
+enum PagedForm { kLine, kLineNt, kPair8, kPair4, kPair4Nt };
 
 template <int D, bool E4>
 static void launch_paged_as(const PAttnK& k, PagedForm form, unsigned grid, hipStream_t s) {
+  constexpr int kPast = E4 ? 1 : 2;
   const dim3 g(grid);
-  if (form == kLine) hipLaunchKernelGGL((paged_attn_kernel<D, E4, false, kLineWaves, true>), g, dim3(64 * kLineWaves), 0, s, k);
-  else if (form == kPair8) hipLaunchKernelGGL((paged_attn_kernel<D, E4, true, 8, false>), g, dim3(512), 0, s, k);
-  else if (form == kPair4) hipLaunchKernelGGL((paged_attn_kernel<D, E4, true, 4, false>), g, dim3(256), 0, s, k);
-  else hipLaunchKernelGGL((paged_attn_kernel<D, E4, true, 4, true>), g, dim3(256), 0, s, k);
+  if (form == kLine) hipLaunchKernelGGL((paged_attn_kernel<D, E4, false, kLineWaves, 1>), g, dim3(64 * kLineWaves), 0, s, k);
+  else if (form == kLineNt) hipLaunchKernelGGL((paged_attn_kernel<D, E4, false, kLineWaves, kPast>), g, dim3(64 * kLineWaves), 0, s, k);
+  else if (form == kPair8) hipLaunchKernelGGL((paged_attn_kernel<D, E4, true, 8, 0>), g, dim3(512), 0, s, k);
+  else if (form == kPair4) hipLaunchKernelGGL((paged_attn_kernel<D, E4, true, 4, 0>), g, dim3(256), 0, s, k);
+  else hipLaunchKernelGGL((paged_attn_kernel<D, E4, true, 4, kPast>), g, dim3(256), 0, s, k);
 }
 
 static void launch_paged(const PAttnK& k, int head_dim, bool e4, PagedForm form, unsigned grid, hipStream_t s) {
@@ -772,7 +808,9 @@ extern "C" int th_paged_attention(const th_paged_attn_desc* d, void* stream) {
     TH_CHECK_LAUNCH();
     return TH_OK;
   }
-  launch_paged(k, d->head_dim, e4, kLine, (unsigned)grid, s);
+  // the most that the call can read: past the last-level cache's size K gains nothing there
+  const int64_t room = std::min(d->pages * d->page_size * d->heads_kv * 2 * d->head_dim * es, pairs * tiles * 16384);
+  launch_paged(k, d->head_dim, e4, room > (256 << 20) ? kLineNt : kLine, (unsigned)grid, s);
   TH_CHECK_LAUNCH();
   // Few pairs can be cut into many parts: a workgroup for each head, and for very
   // few one for each 32 dims of it, reads more of them at once.
