@@ -102,6 +102,26 @@ def test_rope_far_positions(gpu, first):
     assert_within(out.view(t, h, d), ref, (ROT + 2e-6 * (abs(first) > 1 << 30)) * mag + 1e-30)
 
 
+@pytest.mark.parametrize("t,h,d,rot", [((1 << 24) + 5, 1, 6, 2), ((1 << 23) + 5, 33, 64, 64)])
+def test_rope_of_more_workgroups_than_one_dimension_holds(gpu, t, h, d, rot):
+    """A workgroup a token and more tokens than a launch takes along x, in place: the first, the last and those
+    beside the powers of two."""
+    from torch_helion.hip import ops
+
+    announce(f"rope of {t} tokens h={h} d={d}")
+    f = ops.rope_frequencies(rot, 10000.0)
+    ids = torch.tensor([0, 1, (1 << 23) - 1, 1 << 23, t - 6, t - 5, t - 1], device=gpu)
+    x = torch.full((t, h * d), 0.5, dtype=torch.bfloat16, device=gpu)
+    x[ids] = torch.randn(len(ids), h * d, generator=gen(8)).to(torch.bfloat16).to(gpu)
+    pos = torch.arange(t, dtype=torch.int32, device=gpu)
+    before = x[ids].cpu()
+    ops.rope(x, pos, f.to(gpu), x, head_dim=d)
+    ref, mag = rope64(before.view(-1, h, d), pos[ids].cpu(), f)
+    assert_within(x[ids].view(-1, h, d), ref, ROT * mag + u(torch.bfloat16) * ref.abs() + 1e-30)
+    del x
+    torch.cuda.empty_cache()
+
+
 def test_rope_strided_rows_and_a_stream(gpu):
     """Column slices of a wider projection (rows not 16-byte aligned among them), on a side stream."""
     from torch_helion.hip import ops
@@ -549,6 +569,23 @@ def test_copy_pages(gpu, layers, pages, n, ps, hk, d, dtype):
         assert torch.equal(c.view(torch.uint8), r)
     named = torch.tensor([[int(page_map[p]) if 0 <= p < pages else p for p in row] for row in table.tolist()], dtype=torch.int32)
     assert torch.equal(wide[:, :5].cpu(), named) and (wide[:, 5:] == 123456).all()
+
+
+def test_copy_pages_of_more_workgroups_than_one_dimension_holds(gpu):
+    """2^22 + 3 pages of 16 bytes in one layer's two caches: past 2^23 workgroups, and a table renamed behind them."""
+    from torch_helion.hip import ops
+
+    announce("copy of 2^22 + 3 pages")
+    n = (1 << 22) + 3
+    caches = [torch.randint(0, 1 << 14, (2 * n, 1, 1, 8), dtype=torch.int16, device=gpu).view(torch.bfloat16) for _ in range(2)]
+    order = torch.randperm(n, device=gpu)
+    src, dst = order.to(torch.int32), torch.arange(n, 2 * n, dtype=torch.int32, device=gpu)
+    table = torch.arange(2 * n, dtype=torch.int32, device=gpu).view(2, n)
+    ops.copy_pages(*caches, src, dst, page_table=table, page_map=torch.arange(2 * n, dtype=torch.int32, device=gpu).flip(0).contiguous())
+    for c in caches:
+        raw = c.view(torch.int16)
+        assert torch.equal(raw[n:], raw[:n][order])
+    assert torch.equal(table.flatten(), torch.arange(2 * n, dtype=torch.int32, device=gpu).flip(0))
 
 
 def test_copy_pages_skips_what_lies_outside(gpu):

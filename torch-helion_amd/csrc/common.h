@@ -148,4 +148,12 @@ int fp8_scratch_init_device(int device);  // per-device address of th_gemm_noall
 
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// n workgroups along x, and along y where one launch dimension (2^32 threads of
+// 256 a workgroup) does not hold them: workgroup x + y gridDim.x, some past n.
+inline dim3 grid_of(int64_t n) {
+  constexpr int64_t kMost = (int64_t)1 << 23;
+  return n <= kMost ? dim3((unsigned)n) : dim3((unsigned)kMost, (unsigned)cdiv(n, kMost));
+}
+__device__ __forceinline__ int64_t grid_index() { return blockIdx.x + (int64_t)blockIdx.y * gridDim.x; }
+
 }  // namespace th

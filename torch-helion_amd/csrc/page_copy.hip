@@ -26,7 +26,7 @@ struct PageCopyK {
 constexpr int kPiece = 32768;
 
 __global__ void __launch_bounds__(256) page_copy_kernel(PageCopyK p) {
-  int64_t b = blockIdx.x;
+  int64_t b = grid_index();
   if (b >= p.copy_blocks) {  // the workgroups past the copies rename the table
     const int64_t e = (b - p.copy_blocks) * 256 + threadIdx.x;
     if (e >= p.table_entries) return;
@@ -97,7 +97,7 @@ extern "C" int th_page_copy(const th_page_copy_desc* d, void* stream) {
   k.pieces = (int)pieces;
   k.table_entries = entries;
   k.copy_blocks = (int)copies;
-  hipLaunchKernelGGL(page_copy_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, k);
+  hipLaunchKernelGGL(page_copy_kernel, grid_of(blocks), dim3(256), 0, (hipStream_t)stream, k);
   TH_CHECK_LAUNCH();
   return TH_OK;
 }

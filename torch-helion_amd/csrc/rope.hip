@@ -75,9 +75,10 @@ __device__ __forceinline__ bool cache_slot(const RopeK& p, int64_t t, int64_t po
 // of a head at a time, so any head_dim, rot_dim, stride and alignment goes.
 // APPEND: positions are int32, negative ones are skipped, k and v are stored.
 template <typename PosT, typename InT, typename OutT, typename CacheT, bool APPEND>
-__global__ void __launch_bounds__(256) rope_elem_kernel(RopeK p) {
+__global__ void __launch_bounds__(256) rope_elem_kernel(RopeK p, int64_t tokens) {
   __shared__ float cs[kMaxHeadDim / 2], sn[kMaxHeadDim / 2];
-  const int64_t t = blockIdx.x;
+  const int64_t t = grid_index();
+  if (t >= tokens) return;
   const int64_t pos = ((const PosT*)p.positions)[t];
   if (APPEND && pos < 0) return;
   for (int i = threadIdx.x; i < p.half; i += 256) {
@@ -192,7 +193,8 @@ __global__ void __launch_bounds__(256) rope_vec_kernel(RopeK p, int64_t tokens, 
   __shared__ __attribute__((aligned(16))) float cs[kMaxAngles], sn[kMaxAngles];
   __shared__ int64_t slot_k[kMaxTokens], slot_v[kMaxTokens];  // -1: not stored
   __shared__ int live[kMaxTokens];
-  const int64_t t0 = (int64_t)blockIdx.x * tpb;
+  const int64_t t0 = grid_index() * tpb;
+  if (t0 >= tokens) return;
   const int nt = (int)min((int64_t)tpb, tokens - t0);
   const int turns = p.half >> 3, rest = (p.hd - 2 * p.half) >> 3, all = p.hd >> 3;
   const int heads = p.hq + p.hkv;  // hkv is 0 without APPEND
@@ -328,7 +330,7 @@ static void launch_rope(const RopeK& k, int64_t tokens, hipStream_t s) {
           (((uintptr_t)k.kc | (uintptr_t)k.vc) & mask) == 0 && (k.kp | k.kt | k.kh | k.vp | k.vt | k.vh) % 8 == 0;
   }
   if (!vec) {
-    hipLaunchKernelGGL((rope_elem_kernel<PosT, InT, OutT, CacheT, APPEND>), dim3((unsigned)tokens), dim3(256), 0, s, k);
+    hipLaunchKernelGGL((rope_elem_kernel<PosT, InT, OutT, CacheT, APPEND>), grid_of(tokens), dim3(256), 0, s, k, tokens);
     return;
   }
   const int units = (k.hq + k.hkv) * ((k.hd - k.half) >> 3) + k.hkv * (k.hd >> 3);
@@ -340,7 +342,7 @@ static void launch_rope(const RopeK& k, int64_t tokens, hipStream_t s) {
   // 67.5, with the loads alone 74.8.
   const int64_t bytes = tokens * (((int64_t)k.hq + 2 * k.hkv) * k.hd * (int)sizeof(InT) + (int64_t)k.hq * k.hd * (int)sizeof(OutT) +
                                   2 * (int64_t)k.hkv * k.hd * (int)sizeof(CacheT));
-  const dim3 grid((unsigned)cdiv(tokens, tpb));
+  const dim3 grid = grid_of(cdiv(tokens, tpb));
   if (bytes > 128 << 20)
     hipLaunchKernelGGL((rope_vec_kernel<PosT, InT, OutT, CacheT, APPEND, true>), grid, dim3(256), 0, s, k, tokens, tpb);
   else
