@@ -378,7 +378,7 @@ typedef struct th_paged_attn_desc {
   int32_t n_rows, row_pages;
   int64_t pages;
   int32_t window;                       /* 0: none */
-  float scale, softcap;                 /* softcap 0: none; at most 1024 */
+  float scale, softcap;                 /* softcap 0: none, else 2^-20 .. 1024 */
   int32_t pad_;
   const int32_t* positions;             /* [tokens] */
   const int32_t* rows;                  /* optional [tokens] */

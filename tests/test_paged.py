@@ -126,7 +126,7 @@ REFUSED = [
     ("th_paged_attention", attn_desc, [
         ({"heads_q": 5}, "multiple"), ({"head_dim": 96}, "head_dim"), ({"cache_dtype": 0}, "cache_dtype"), ({"page_size": 8}, "page_size"),
         ({"page_size": 48}, "page_size"), ({"row_pages": 0}, "page table"), ({"window": -1}, "window"), ({"softcap": -1.0}, "softcap"),
-        ({"softcap": float("nan")}, "softcap"), ({"softcap": 1025.0}, "softcap"), ({"tokens": 65536}, "tokens"), ({"ld_q": 255}, "row strides"), ({"ld_q": 260}, "16 bytes"),
+        ({"softcap": float("nan")}, "softcap"), ({"softcap": 1025.0}, "softcap"), ({"softcap": 1e-39}, "softcap"), ({"tokens": 65536}, "tokens"), ({"ld_q": 255}, "row strides"), ({"ld_q": 260}, "16 bytes"),
         ({"k_stride_h": 68}, "16 bytes"), ({"v_stride_page": 2050}, "16 bytes"), ({"cache_dtype": 3, "k_stride_t": 136}, "16 bytes"),
         ({"k_stride_t": 1 << 23}, "token strides"), ({"q": 16392}, "16-byte"), ({"v_cache": 65544}, "16-byte"), ({"v_scale": 4096}, "e4m3"),
         ({"tokens": -1}, "tokens"), ({"tokens": 5}, "exceed the table"), ({"positions": 0}, "null"), ({"o": 0}, "null"),
@@ -230,7 +230,7 @@ def test_more_argument_checks():
             (append, {"v": a["v"].float()}, "v must be"), (append, {"q": a["q"]}, "q_out"), (append, {"freqs": a["freqs"].float()}, "freqs"),
             (append, {"k": a["k"][:, :64]}, "k must be"), (append, {"k": a["k"][:1].expand(4, -1)}, "row stride|HIP device"),
             (append, {"q": a["q"][:, :100], "q_out": a["q"]}, "heads"), (attend, {"q": a["q"].float()}, "q must be .* torch.bfloat16"),
-            (attend, {"slopes": torch.ones(3)}, "slopes"), (attend, {"out": a["out"][:3]}, "out must be"),
+            (attend, {"slopes": torch.ones(3)}, "slopes"), (attend, {"window": 1 << 32}, "window"), (attend, {"window": -1}, "window"), (attend, {"out": a["out"][:3]}, "out must be"),
             (rope, {"head_dim": 60}, "heads"), (rope, {"positions": a["positions"].float()}, "int32 or int64"),
             (rope, {"out": a["out"].float()}, "out must be"), (rope, {}, "HIP device"), (copy, {"src": a["positions"][:2]}, "dst"),
             (copy, {"page_table": a["page_table"]}, "page_map"), (copy, {"k_cache": a["k_cache"][:, :8], "v_cache": a["v_cache"][:, :8]}, "HIP device"),

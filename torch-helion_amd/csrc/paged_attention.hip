@@ -721,7 +721,7 @@ extern "C" int64_t th_paged_attention_workspace_bytes(int32_t tokens, int32_t he
       (cache_dtype != TH_BF16 && cache_dtype != TH_F8E4M3) || max_keys <= 0 || max_keys >= (int64_t)1 << 30 || window < 0)
     return -1;
   const int g = heads_q / heads_kv, row_bytes = head_dim * (cache_dtype == TH_BF16 ? 2 : 1);
-  if (tokens == 0 || pair_form(most_tiles(max_keys, window, row_bytes), tokens * heads_kv * cdiv(g, 16))) return 0;
+  if (tokens == 0 || pair_form(most_tiles(max_keys, window, row_bytes), (int64_t)tokens * heads_kv * cdiv(g, 16))) return 0;
   const int64_t gq = std::min(g, 16), slots = (int64_t)line_grid() * kLineWaves * 2;
   return cdiv((int64_t)(tokens + 1) * 8, 16) * 16 + cdiv(slots * gq * 2 * 4, 16) * 16 + slots * gq * head_dim * 4;
 }
@@ -741,8 +741,9 @@ extern "C" int th_paged_attention(const th_paged_attn_desc* d, void* stream) {
   TH_CHECK_ARG((int64_t)d->row_pages * d->page_size < (int64_t)1 << 30, "th_paged_attention: row of 2^30 keys or more");
   // The capped score's error is 1e-7 of the cap (its tanh is 1 - 2 / (1 + e^2x)): up
   // to here 1e-4, a fortieth of what rounding p to bf16 does.
-  TH_CHECK_ARG(d->window >= 0 && d->softcap >= 0.f && d->softcap <= 1024.f,
-               "th_paged_attention: window %d must not be negative, softcap %g in 0..1024", d->window, (double)d->softcap);
+  TH_CHECK_ARG(d->window >= 0 && (d->softcap == 0.f || (d->softcap >= 0x1p-20f && d->softcap <= 1024.f)),
+               "th_paged_attention: window %d must not be negative, softcap %g 0 or in 2^-20..1024", d->window,
+               (double)d->softcap);
   const int64_t row = (int64_t)d->heads_q * d->head_dim;
   TH_CHECK_ARG(d->ld_q >= row && d->ld_o >= row, "th_paged_attention: q/o row strides smaller than heads_q*head_dim");
   const int per = d->cache_dtype == TH_BF16 ? 8 : 16;  // elements in 16 bytes
@@ -808,7 +809,7 @@ extern "C" int th_paged_attention(const th_paged_attn_desc* d, void* stream) {
     TH_CHECK_LAUNCH();
     return TH_OK;
   }
-  // the most that the call can read: past the last-level cache's size K gains nothing there
+  // the most that the call can read: K goes past the caches where that does not fit them
   const int64_t room = std::min(d->pages * d->page_size * d->heads_kv * 2 * d->head_dim * es, pairs * tiles * 16384);
   launch_paged(k, d->head_dim, e4, room > (256 << 20) ? kLineNt : kLine, (unsigned)grid, s);
   TH_CHECK_LAUNCH();

@@ -500,8 +500,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     tokens; ``out`` may be ``q``. head_dim is 64 or 128, the pages hold 16 tokens or more.
 
     The token at position p sees the keys 0 .. p of its row, the last ``window`` of them if given.
-    Scores are ``scale q . k``, capped as ``softcap tanh(s / softcap)`` if given (at most 1024), then biased by
-    ``-slopes[h] (p - j)`` (fp32 [heads_q]) if given. A token without keys gets zeros.
+    Scores are ``scale q . k``, capped as ``softcap tanh(s / softcap)`` if given (2^-20 to
+    1024), then biased by ``-slopes[h] (p - j)`` (fp32 [heads_q]) if given. A token without keys gets zeros.
     ``workspace``: :func:`paged_attention_workspace_bytes` bytes that no concurrent call uses;
     without one the call takes it from torch's allocator. A table cut to the pages in use
     (``page_table[:, :n]``) lets short rows take a faster form."""
@@ -510,6 +510,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     (pages, page_size, hk, hd), ks, vs = _cache(k_cache, v_cache, dev, entry)
     shape = n, width = _heads(q, hd, entry, "q")
     hq = width // hd
+    if not 0 <= window < 1 << 31:
+        _refuse(entry, f"window {window} out of range")
     n_rows, row_pages, pos, rp, tp, ldt = _places(page_table, positions, rows, n, dev, entry)
     sq, so = q.stride(), out.stride()
     if not (q.dtype is torch.bfloat16 and sq[1] == 1 and out.shape == shape and out.dtype is torch.bfloat16 and so[1] == 1

@@ -314,13 +314,15 @@ class PagedDecodeBlock(DecodeBlock):
         with torch.cuda.device(self.device):
             held = positions.clone()
             positions.fill_(-1)
-            torch.cuda.synchronize()
-            self.step(x, positions, rows)
-            torch.cuda.synchronize()
-            g = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(g):
+            try:
+                torch.cuda.synchronize()
                 self.step(x, positions, rows)
-            positions.copy_(held)
+                torch.cuda.synchronize()
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g):
+                    self.step(x, positions, rows)
+            finally:
+                positions.copy_(held)
             torch.cuda.synchronize()
         self.graph = g
 
