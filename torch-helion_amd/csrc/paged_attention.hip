@@ -62,6 +62,7 @@ struct PAttnK {
   int tokens, Hkv, G, nqb, gq;  // nqb blocks of gq <= 16 query heads per kv head
   int window;
   int o8;           // o in whole 8-byte pieces
+  int turn;         // pair: workgroups that give each XCD one token (0: no order)
   float scale, softcap;
   const float* slopes;
   const float* ks;
@@ -174,7 +175,7 @@ __device__ __forceinline__ void keep_step(int64_t step) {
 // (pair form) 17.0, 19.5, 20.1, 64 short lines (82 MB) 25.2, 26.3, 27.6; caches of
 // that size that are not there yet, 16 sequences of 500-4000 keys: 40.2, 37.2, 37.9.
 template <int D, bool E4, bool PAIR, int NW, int NT>
-__global__ void __launch_bounds__(64 * NW, 8 / NW) paged_attn_kernel(PAttnK p) {
+__global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2))) paged_attn_kernel(PAttnK p) {
   using T = PaTile<D, E4>;
   constexpr int KU = PAIR ? NW * T::KT : T::KT;  // keys of a step: of the workgroup's, or of one wave's
   constexpr int RB = T::RB, KT = T::KT, NB = T::NB, CPR = T::CPR, RPI = T::RPI;
@@ -193,6 +194,10 @@ __global__ void __launch_bounds__(64 * NW, 8 / NW) paged_attn_kernel(PAttnK p) {
   Span sp;
   if constexpr (PAIR) {
     me = blockIdx.x;
+    if (p.turn) {  // the heads of a token on one XCD (workgroups go to the eight in turn)
+      const int at = me / p.turn * p.turn, i = me - at;
+      if (at + p.turn <= (int)gridDim.x) me = at + (i & 7) * HB + (i >> 3);
+    }
     t = me / HB;
     hb = me - t * HB;
     k = 0;
@@ -668,26 +673,28 @@ __global__ void __launch_bounds__(256) paged_attn_join_kernel(PAttnK p, int wave
   for (int r = 0; r < 4; ++r) o[c * D + d0 + 4 * ln + r] = f32_to_bf16(x[r] * f);
 }
 
-enum PagedForm { kLine, kLineNt, kPair8, kPair4, kPair4Nt };
-
+// pair: 0, the line form, or the waves of a pair's workgroup. nt: past the caches.
 template <int D, bool E4>
-static void launch_paged_as(const PAttnK& k, PagedForm form, unsigned grid, hipStream_t s) {
+static void launch_paged_as(const PAttnK& k, int pair, bool nt, unsigned grid, hipStream_t s) {
   constexpr int kPast = E4 ? 1 : 2;
-  const dim3 g(grid);
-  if (form == kLine) hipLaunchKernelGGL((paged_attn_kernel<D, E4, false, kLineWaves, 1>), g, dim3(64 * kLineWaves), 0, s, k);
-  else if (form == kLineNt) hipLaunchKernelGGL((paged_attn_kernel<D, E4, false, kLineWaves, kPast>), g, dim3(64 * kLineWaves), 0, s, k);
-  else if (form == kPair8) hipLaunchKernelGGL((paged_attn_kernel<D, E4, true, 8, 0>), g, dim3(512), 0, s, k);
-  else if (form == kPair4) hipLaunchKernelGGL((paged_attn_kernel<D, E4, true, 4, 0>), g, dim3(256), 0, s, k);
-  else hipLaunchKernelGGL((paged_attn_kernel<D, E4, true, 4, kPast>), g, dim3(256), 0, s, k);
+  const dim3 g(grid), b(64 * (pair ? pair : kLineWaves));
+  if (pair == 0 && nt) hipLaunchKernelGGL((paged_attn_kernel<D, E4, false, kLineWaves, kPast>), g, b, 0, s, k);
+  else if (pair == 0) hipLaunchKernelGGL((paged_attn_kernel<D, E4, false, kLineWaves, 1>), g, b, 0, s, k);
+  else if (pair == 8) hipLaunchKernelGGL((paged_attn_kernel<D, E4, true, 8, 0>), g, b, 0, s, k);
+  else if (pair == 4 && nt) hipLaunchKernelGGL((paged_attn_kernel<D, E4, true, 4, kPast>), g, b, 0, s, k);
+  else if (pair == 4) hipLaunchKernelGGL((paged_attn_kernel<D, E4, true, 4, 0>), g, b, 0, s, k);
+  else if (pair == 2) hipLaunchKernelGGL((paged_attn_kernel<D, E4, true, 2, 0>), g, b, 0, s, k);
+  else if (nt) hipLaunchKernelGGL((paged_attn_kernel<D, E4, true, 1, kPast>), g, b, 0, s, k);
+  else hipLaunchKernelGGL((paged_attn_kernel<D, E4, true, 1, 0>), g, b, 0, s, k);
 }
 
-static void launch_paged(const PAttnK& k, int head_dim, bool e4, PagedForm form, unsigned grid, hipStream_t s) {
+static void launch_paged(const PAttnK& k, int head_dim, bool e4, int pair, bool nt, unsigned grid, hipStream_t s) {
   if (head_dim == 128) {
-    if (e4) launch_paged_as<128, true>(k, form, grid, s);
-    else launch_paged_as<128, false>(k, form, grid, s);
+    if (e4) launch_paged_as<128, true>(k, pair, nt, grid, s);
+    else launch_paged_as<128, false>(k, pair, nt, grid, s);
   } else {
-    if (e4) launch_paged_as<64, true>(k, form, grid, s);
-    else launch_paged_as<64, false>(k, form, grid, s);
+    if (e4) launch_paged_as<64, true>(k, pair, nt, grid, s);
+    else launch_paged_as<64, false>(k, pair, nt, grid, s);
   }
 }
 
@@ -707,13 +714,30 @@ static int64_t most_tiles(int64_t max_keys, int window, int row_bytes) {
 // Whether pairs take the pair form. In a graph, us, pair against line form, lengths
 // of half to all of the room (bf16, 128 dims, 8 kv heads, 4 query heads each):
 //   tiles of room      16            32            64
-//     8 pairs       9.8 /  9.8   14.5 / 10.6   23.6 / 10.5
-//   128 pairs      10.8 / 15.0   16.2 / 20.9   26.2 / 29.0
-//   512 pairs      20.4 / 28.8   42.0 / 50.0   80.1 / 85.4
-//  2048 pairs      79.3 / 92.8    147 /  160    286 /  288
+//     8 pairs       6.4 /  8.9    7.9 /  9.0   11.1 /  9.3
+//   128 pairs       9.8 / 14.5   14.7 / 20.6   23.5 / 28.0
+//   512 pairs      20.5 / 28.6   39.0 / 43.1   75.9 / 76.8
+//  2048 pairs      69.0 / 80.7    130 /  142    255 /  259
+// and with an e4m3 cache at 32 tiles 10.5 / 9.5 for 8 pairs, 18.4 / 22.3 for 128.
 // 64 tiles and more stay with the line: lengths are not known here, and one full
-// row among short ones would cost the pair form 24 us where the line takes 10.
+// row among short ones would cost the pair form 20 us where the line takes 9.
 static bool pair_form(int64_t tiles, int64_t pairs) { return tiles <= 16 || (tiles <= 32 && pairs >= 128); }
+
+// Waves of a pair's workgroup: as many as the pair can have tiles, while the CUs
+// (eight waves each) hold all pairs at once. us with 4, 2, 1 waves, bf16, 128 dims:
+//   tiles of room          1                  2                   4                   8
+//   512 pairs       5.9  5.3  5.1      6.1  5.7  6.5      8.8  9.0 10.4     12.3 13.3 16.7
+//   768 pairs       9.0  5.6  5.3      9.8  7.1  8.0     12.9 10.8 12.3     17.9 16.2 18.9
+//  2048 pairs      18.6 12.6  8.9     19.8 15.1 13.0     23.9 21.9 20.2     40.8 42.8 41.3
+// Past 8 tiles 8 waves where there is a CU for each pair (256 pairs, 16 tiles of
+// e4m3: 16.1 against 16.7 with 4, 32 tiles 24.1 against 27.5), else 4.
+static int pair_waves(int64_t tiles, int64_t pairs) {
+  const int64_t cus = line_grid();
+  if (tiles > 8) return pairs <= cus ? 8 : 4;
+  int w = tiles > 2 ? 4 : (int)tiles;
+  while (w > 1 && pairs * w > 8 * cus) w >>= 1;
+  return w;
+}
 
 extern "C" int64_t th_paged_attention_workspace_bytes(int32_t tokens, int32_t heads_q, int32_t heads_kv, int32_t head_dim,
                                                        int32_t cache_dtype, int64_t max_keys, int32_t window) {
@@ -801,17 +825,20 @@ extern "C" int th_paged_attention(const th_paged_attn_desc* d, void* stream) {
   const int64_t pairs = (int64_t)d->tokens * d->heads_kv * k.nqb;  // below 2^24
   const int64_t tiles = most_tiles((int64_t)d->row_pages * d->page_size, d->window, (int)(d->head_dim * es));
   if (pair_form(tiles, pairs)) {
-    // eight waves where there is a CU for each pair and they have more than a tile
-    // each (256 pairs, 16 tiles of e4m3: 16.1 us against 16.7, 32 tiles 24.1 against
-    // 27.5), else four (4 tiles 6.2 against 7.0; 512 pairs would wait for CUs)
-    const PagedForm form = pairs <= device_cus() && tiles > 8 ? kPair8 : pairs * tiles > (128 << 20) / 16384 ? kPair4Nt : kPair4;
-    launch_paged(k, d->head_dim, e4, form, (unsigned)pairs, s);
+    // Heads of a token side by side on one XCD, whose L2 they share: where a row is half
+    // a 128-byte line (the other half is the next head's), and from 512 MB on, where
+    // neighbours are read together. us, in order and so: 64-byte rows of 512 pairs, 16
+    // tiles 37.7 / 26.7, of 5600 pairs, 32 tiles 683 / 476; 128-byte rows of 2048 pairs,
+    // 32 tiles 152 / 142, of 5600 pairs 389 / 342; 256-byte rows 134 / 135, 353 / 347;
+    // smaller calls lose 2 to 5 percent: 512 pairs, 16 tiles 21.7 / 23.3.
+    k.turn = d->head_dim * es < 128 || pairs * tiles >= (512 << 20) / 16384 ? 8 * d->heads_kv * k.nqb : 0;
+    launch_paged(k, d->head_dim, e4, pair_waves(tiles, pairs), pairs * tiles > (128 << 20) / 16384, (unsigned)pairs, s);
     TH_CHECK_LAUNCH();
     return TH_OK;
   }
   // the most that the call can read: K goes past the caches where that does not fit them
   const int64_t room = std::min(d->pages * d->page_size * d->heads_kv * 2 * d->head_dim * es, pairs * tiles * 16384);
-  launch_paged(k, d->head_dim, e4, room > (256 << 20) ? kLineNt : kLine, (unsigned)grid, s);
+  launch_paged(k, d->head_dim, e4, 0, room > (256 << 20), (unsigned)grid, s);
   TH_CHECK_LAUNCH();
   // Few pairs can be cut into many parts: a workgroup for each head, and for very
   // few one for each 32 dims of it, reads more of them at once.
