@@ -491,6 +491,24 @@ def test_attention_short_rows_in_long_tables(gpu, lens, hq, hk, d, ps, cache):
     check_attention(gpu, lens, hq, hk, d, ps, cache=cache, row_pages=8192 // ps, poison=len(lens) < 100)
 
 
+@pytest.mark.parametrize("tokens,hq,hk,d,room,cache", [
+    (70, 16, 8, 128, 64, BF16),      # 560 pairs of two tiles: two waves
+    (150, 8, 8, 64, 64, BF16),       # 1200 pairs of one tile: one wave
+    (139, 16, 8, 128, 128, BF16),    # 1112 pairs of four tiles: one wave, four tiles in turn
+    (21, 6, 3, 64, 512, E4M3),       # 64-byte rows: an XCD takes a token, the last five in order
+    (300, 4, 4, 64, 128, E4M3),
+    (275, 8, 8, 64, 1024, BF16),     # from 512 MB of room on: 2200 pairs of 16 tiles
+    (260, 32, 16, 128, 256, E4M3),   # 4160 pairs of 4 tiles past the caches
+    (1100, 8, 8, 64, 512, E4M3),     # 8800 pairs of 4 tiles: one wave, tokens to the XCDs in turn
+])
+def test_attention_many_pairs(gpu, tokens, hq, hk, d, room, cache):
+    """Every number of waves a pair can get and both orders of the pairs; few pages hold the keys of all."""
+    announce(f"paged attention, {tokens} tokens of {hk} kv heads d={d} room={room} {cache}")
+    rows = [i % 7 for i in range(tokens)]
+    lens = [1 + (37 * i) % room for i in range(tokens)]
+    check_attention(gpu, lens, hq, hk, d, 16, rows=rows, cache=cache, row_pages=room // 16, poison=False, seed=tokens)
+
+
 def test_attention_many_tokens_of_one_row(gpu):
     """700 tokens of one row (a prompt's tail): several tokens to each run of the line's prefix sums."""
     announce("paged attention, 700 tokens of a row")
