@@ -231,7 +231,7 @@ def test_more_argument_checks():
             (append, {"k": a["k"][:, :64]}, "k must be"), (append, {"k": a["k"][:1].expand(4, -1)}, "row stride|HIP device"),
             (append, {"q": a["q"][:, :100], "q_out": a["q"]}, "heads"), (attend, {"q": a["q"].float()}, "q must be .* torch.bfloat16"),
             (attend, {"slopes": torch.ones(3)}, "slopes"), (attend, {"window": 1 << 32}, "window"), (attend, {"window": -1}, "window"), (attend, {"out": a["out"][:3]}, "out must be"),
-            (rope, {"head_dim": 60}, "heads"), (rope, {"positions": a["positions"].float()}, "int32 or int64"),
+            (rope, {"head_dim": 60}, "heads"), (rope, {"scale": 1e40}, "out of range"), (rope, {"positions": a["positions"].float()}, "int32 or int64"),
             (rope, {"out": a["out"].float()}, "out must be"), (rope, {}, "HIP device"), (copy, {"src": a["positions"][:2]}, "dst"),
             (copy, {"page_table": a["page_table"]}, "page_map"), (copy, {"k_cache": a["k_cache"][:, :8], "v_cache": a["v_cache"][:, :8]}, "HIP device"),
             (copy, {"k_cache": a["k_cache"][:, ::2], "v_cache": a["v_cache"][:, ::2]}, "dense"), (copy, {}, "HIP device")):

@@ -9,6 +9,7 @@ the HIP runtime torch has already mapped.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from pathlib import Path
 
 from .build import LIB_PATH
@@ -195,7 +196,17 @@ class VmDesc(C.Structure):
     ]
 
 
-# entry point name -> (restype, argtypes); every symbol include/th_hip.h declares
+def packer(desc: type[C.Structure]) -> struct.Struct:
+    """Packs all the fields of a descriptor (no padding, no arrays) into the bytes that an entry point reads:
+    0.65 us for 34 fields, a Structure takes 1.6. Pointers are ints, 0 for none."""
+    codes = {_i32: "i", _i64: "q", C.c_float: "f", _p: "Q"}
+    s = struct.Struct("=" + "".join(codes[kind] for _, kind in desc._fields_))
+    assert s.size == C.sizeof(desc)
+    return s
+
+
+# entry point name -> (restype, argtypes); every symbol include/th_hip.h declares. A descriptor
+# that a packer fills is passed as its bytes.
 SIGNATURES: dict[str, tuple] = {
     "th_abi_version": (_i32, []),
     "th_init": (_i32, [_i32]),
@@ -211,11 +222,11 @@ SIGNATURES: dict[str, tuple] = {
     "th_attention_prefill": (_i32, [C.POINTER(AttnDesc), _p]),
     "th_attention_decode_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32]),
     "th_attention_decode": (_i32, [C.POINTER(DecodeDesc), _p]),
-    "th_rope": (_i32, [C.POINTER(RopeDesc), _p]),
-    "th_paged_append": (_i32, [C.POINTER(PagedAppendDesc), _p]),
+    "th_rope": (_i32, [_p, _p]),
+    "th_paged_append": (_i32, [_p, _p]),
     "th_paged_attention_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i64, _i32]),
-    "th_paged_attention": (_i32, [C.POINTER(PagedAttnDesc), _p]),
-    "th_page_copy": (_i32, [C.POINTER(PageCopyDesc), _p]),
+    "th_paged_attention": (_i32, [_p, _p]),
+    "th_page_copy": (_i32, [_p, _p]),
     "th_epilogue_vm": (_i32, [C.POINTER(VmDesc), _p]),
     "th_ssd_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32]),
     "th_ssd_gtile_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),

@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import math
+import struct
 from dataclasses import dataclass, field
 from typing import Sequence
 
@@ -288,7 +289,17 @@ def _refuse(entry: str, message: str) -> None:
     raise abi.HipBackendError(entry, abi.TH_ERR_INVALID, message)
 
 
-def _launch(entry: str, desc: C.Structure, dev: int, kernel: str | None) -> None:
+_ROPE, _APPEND, _ATTEND, _COPY = (abi.packer(d) for d in (abi.RopeDesc, abi.PagedAppendDesc, abi.PagedAttnDesc, abi.PageCopyDesc))
+
+
+def _pack(entry: str, packer: struct.Struct, *values) -> bytes:
+    try:
+        return packer.pack(*values)
+    except (struct.error, OverflowError) as e:   # a size past its 32 or 64 bits, a float past its range
+        raise abi.HipBackendError(entry, abi.TH_ERR_INVALID, f"argument out of range: {e}") from None
+
+
+def _launch(entry: str, desc: bytes, dev: int, kernel: str | None) -> None:
     """One library call on the current stream of device ``dev`` (a tensor's get_device()), whichever
     device is current."""
     if dev < 0:
@@ -297,7 +308,7 @@ def _launch(entry: str, desc: C.Structure, dev: int, kernel: str | None) -> None
         with torch.cuda.device(dev):
             return _launch(entry, desc, dev, kernel)
     lib = abi.init_device(dev)
-    status = getattr(lib, entry)(C.byref(desc), torch._C._cuda_getCurrentRawStream(dev))
+    status = getattr(lib, entry)(desc, torch._C._cuda_getCurrentRawStream(dev))
     if status != abi.TH_OK:
         abi.check(status, entry, kernel)
 
@@ -392,8 +403,8 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, out: tor
         _rows_of(out, n, width, dt, dev, entry, "out")
         _vector(positions, n, pt, dev, entry, "positions")
         _vector(freqs, half, torch.float64, dev, entry, "freqs")
-    d = abi.RopeDesc(n, width // head_dim, head_dim, 2 * half, interleaved, inverse, th_dtype(dt), _DT[pt], scale,
-                     x.data_ptr(), _ld(sx, shape), positions.data_ptr(), freqs.data_ptr(), out.data_ptr(), _ld(so, shape))
+    d = _pack(entry, _ROPE, n, width // head_dim, head_dim, 2 * half, interleaved, inverse, th_dtype(dt), _DT[pt], scale,
+              x.data_ptr(), _ld(sx, shape), positions.data_ptr(), freqs.data_ptr(), out.data_ptr(), _ld(so, shape))
     _launch(entry, d, dev, kernel)
     return out
 
@@ -420,7 +431,7 @@ def _places(page_table: torch.Tensor, positions: torch.Tensor, rows: torch.Tenso
             _refuse(entry, "page_table must be int32 [rows, pages per row]")
         _rows_of(page_table, shape[0], shape[1], torch.int32, dev, entry, "page_table")
         _vector(positions, n, torch.int32, dev, entry, "positions")
-    return (shape[0], shape[1], positions.data_ptr(), None if rows is None else _vector(rows, n, torch.int32, dev, entry, "rows"),
+    return (shape[0], shape[1], positions.data_ptr(), 0 if rows is None else _vector(rows, n, torch.int32, dev, entry, "rows"),
             page_table.data_ptr(), _ld(strides, shape))
 
 
@@ -448,11 +459,11 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, k_ca
     if not (k.shape == shape and v.shape == shape and v.dtype is dt and sk[1] == 1 and sv[1] == 1 and v.get_device() == dev):
         _rows_of(k, n, width, dt, dev, entry, "k")
         _rows_of(v, n, width, dt, dev, entry, "v")
-    half, fp = 0, None
+    half = fp = 0
     if freqs is not None:
         half = freqs.numel()
         fp = _vector(freqs, half, torch.float64, dev, entry, "freqs")
-    hq, qp, ldq, op, ldo = 0, None, 0, None, 0
+    hq = qp = ldq = op = ldo = 0
     if q is not None:
         if q_out is None:
             _refuse(entry, "q needs a q_out")
@@ -462,13 +473,13 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, k_ca
             _rows_of(q, n, shape_q[1], dt, dev, entry, "q")
             _rows_of(q_out, n, shape_q[1], torch.bfloat16, dev, entry, "q_out")
         hq, qp, ldq, op, ldo = shape_q[1] // hd, q.data_ptr(), _ld(sq, shape_q), q_out.data_ptr(), _ld(so, shape_q)
-    d = abi.PagedAppendDesc(
-        n, hq, hk, hd, 2 * half, interleaved, th_dtype(dt), th_dtype(k_cache.dtype), page_size, n_rows, row_pages, pages,
-        rope_scale, 0, pos, rp, tp, ldt, fp, qp, ldq, op, ldo, k.data_ptr(), _ld(sk, shape), v.data_ptr(), _ld(sv, shape),
+    d = _pack(
+        entry, _APPEND, n, hq, hk, hd, 2 * half, interleaved, th_dtype(dt), th_dtype(k_cache.dtype), page_size, n_rows, row_pages,
+        pages, rope_scale, 0, pos, rp, tp, ldt, fp, qp, ldq, op, ldo, k.data_ptr(), _ld(sk, shape), v.data_ptr(), _ld(sv, shape),
         k_cache.data_ptr(), ks[0], ks[1], ks[2], v_cache.data_ptr(), vs[0], vs[1], vs[2],
-        None if k_scale is None else _vector(k_scale, hk, torch.float32, dev, entry, "k_scale"),
-        None if v_scale is None else _vector(v_scale, hk, torch.float32, dev, entry, "v_scale"),
-        None if n_invalid is None else _vector(n_invalid, 1, torch.int32, dev, entry, "n_invalid"))
+        0 if k_scale is None else _vector(k_scale, hk, torch.float32, dev, entry, "k_scale"),
+        0 if v_scale is None else _vector(v_scale, hk, torch.float32, dev, entry, "v_scale"),
+        0 if n_invalid is None else _vector(n_invalid, 1, torch.int32, dev, entry, "n_invalid"))
     _launch(entry, d, dev, kernel)
 
 
@@ -518,7 +529,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             and out.get_device() == dev):
         _rows_of(q, n, width, torch.bfloat16, dev, entry, "q")
         _rows_of(out, n, width, torch.bfloat16, dev, entry, "out")
-    wp, wn = None, 0
+    wp = wn = 0
     if workspace is not None:
         if workspace.get_device() != dev or not workspace.is_contiguous():
             _refuse(entry, f"workspace must be a contiguous tensor on {_place(dev)}")
@@ -528,12 +539,12 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         if wn:
             workspace = torch.empty(wn, dtype=torch.uint8, device=q.device)
             wp = workspace.data_ptr()
-    d = abi.PagedAttnDesc(
-        n, hq, hk, hd, th_dtype(k_cache.dtype), page_size, n_rows, row_pages, pages, window, scale, softcap, 0, pos, rp, tp, ldt,
-        q.data_ptr(), _ld(sq, shape), k_cache.data_ptr(), ks[0], ks[1], ks[2], v_cache.data_ptr(), vs[0], vs[1], vs[2],
-        None if slopes is None else _vector(slopes, hq, torch.float32, dev, entry, "slopes"),
-        None if k_scale is None else _vector(k_scale, hk, torch.float32, dev, entry, "k_scale"),
-        None if v_scale is None else _vector(v_scale, hk, torch.float32, dev, entry, "v_scale"), out.data_ptr(), _ld(so, shape), wp, wn)
+    d = _pack(
+        entry, _ATTEND, n, hq, hk, hd, th_dtype(k_cache.dtype), page_size, n_rows, row_pages, pages, window, scale, softcap, 0, pos,
+        rp, tp, ldt, q.data_ptr(), _ld(sq, shape), k_cache.data_ptr(), ks[0], ks[1], ks[2], v_cache.data_ptr(), vs[0], vs[1], vs[2],
+        0 if slopes is None else _vector(slopes, hq, torch.float32, dev, entry, "slopes"),
+        0 if k_scale is None else _vector(k_scale, hk, torch.float32, dev, entry, "k_scale"),
+        0 if v_scale is None else _vector(v_scale, hk, torch.float32, dev, entry, "v_scale"), out.data_ptr(), _ld(so, shape), wp, wn)
     _launch(entry, d, dev, kernel)
     return out
 
@@ -564,7 +575,7 @@ def copy_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, src: torch.Tensor, 
                     _refuse(entry, f"a page of the {name} cache must be one dense block, got strides {strides}")
                 run *= extent
         operands += [t.data_ptr(), strides[0] * size if layered else 0, strides[-4] * size]
-    table = (None, 0, 0, 0, None)
+    table = (0, 0, 0, 0, 0)
     if page_table is not None:
         if page_map is None:
             _refuse(entry, "renaming a page_table needs a page_map")
@@ -573,8 +584,8 @@ def copy_pages(k_cache: torch.Tensor, v_cache: torch.Tensor, src: torch.Tensor, 
         rows, width = page_table.shape
         tp, ldt = _rows_of(page_table, rows, width, torch.int32, dev, entry, "page_table")
         table = (tp, ldt, rows, width, _vector(page_map, pages, torch.int32, dev, entry, "page_map"))
-    d = abi.PageCopyDesc(shape[0] if layered else 1, n, pages, page, *operands,
-                         _vector(src, n, torch.int32, dev, entry, "src"), _vector(dst, n, torch.int32, dev, entry, "dst"), *table)
+    d = _pack(entry, _COPY, shape[0] if layered else 1, n, pages, page, *operands,
+              _vector(src, n, torch.int32, dev, entry, "src"), _vector(dst, n, torch.int32, dev, entry, "dst"), *table)
     _launch(entry, d, dev, kernel)
 
 
