@@ -37,9 +37,9 @@
 //   O^T      += V^T P^T: V is read transposed (ds_read_b64_tr_b16); P^T is the S^T
 //            accumulators as they are, rounded to bf16 (half a step is 2^-8 of each
 //            p; sums and maxima stay fp32).
-// The next tile's loads are issued as soon as V is staged, and land during the
-// softmax and the second product. Buffer loads return zero past their
-// range: unseen slots of a page and pages outside the cache cost no branch, and
+// The next tile's loads are issued as soon as this one has left its registers, and
+// land during the softmax and the second product. Buffer loads return zero past
+// their range: unseen slots of a page and pages outside the cache cost no branch, and
 // whatever they hold (NaN) never meets a zero probability.
 #include "common.h"
 
