@@ -27,7 +27,7 @@
 //
 // One tile:
 //   V        loaded by whole rows (16-byte pieces, consecutive lanes next to each
-//            other) and staged as bf16 in the wave's own LDS slice, swizzled.
+//            other) and staged in 16 bits in the wave's own LDS slice, swizzled.
 //   S^T      = K Q^T, v_mfma_f32_16x16x32_bf16: lane l supplies row l % 16 and 8
 //            dims from 8 (l / 16). A bf16 K goes through the slice too, before V:
 //            loaded in its operand layout, half a 128-byte line of 16 rows at a
@@ -35,8 +35,14 @@
 //            K is loaded in that layout, the dims of a row permuted (16 consecutive
 //            ones serve two k steps, q alike): 100.3 us, through the slice 101.6.
 //   O^T      += V^T P^T: V is read transposed (ds_read_b64_tr_b16); P^T is the S^T
-//            accumulators as they are, rounded to bf16 (half a step is 2^-8 of each
-//            p; sums and maxima stay fp32).
+//            accumulators as they are, sums and maxima stay fp32. With a bf16 V each
+//            p goes in as two bf16 halves, h + (p - h): off by 2^-16 of it. One half
+//            (2^-8) took the error against 64 bits from 0.0017, the output's own
+//            rounding, to 0.0020-0.0022, for 133.2 us instead of 133.8 (64 sequences
+//            of 2048-4096 keys), 17.1 instead of 17.7 (23 windows of 1000, 12 heads of
+//            64). An e4m3 V is staged as fp16, which holds it exactly, and p is one
+//            fp16 (2^-11: error 0.0017): 95.9 us, as with one bf16 half (0.0021); two
+//            halves 100.3.
 // The next tile's loads are issued as soon as this one has left its registers, and
 // land during the softmax and the second product. Buffer loads return zero past
 // their range: unseen slots of a page and pages outside the cache cost no branch, and
@@ -46,6 +52,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace th {
 
@@ -76,6 +83,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 typedef unsigned pa_u32x4 __attribute__((ext_vector_type(4)));
 typedef short pa_s16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ void pa_lds_order() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -135,12 +143,23 @@ __device__ __forceinline__ bf16x8_t e4m3x8_to_bf16(unsigned lo, unsigned hi) {
   return u.v;
 }
 
+// The same as 8 fp16: exact too.
+__device__ __forceinline__ f16x8_t e4m3x8_to_f16(unsigned lo, unsigned hi) {
+  typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+  union { h2_t h[4]; f16x8_t v; } u;
+  u.h[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false);
+  u.h[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true);
+  u.h[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false);
+  u.h[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true);
+  return u.v;
+}
+
 // LDS slot of 16-byte chunk c of K row r is c ^ ksw(r): the 16 rows of an operand
 // read then hit distinct banks.
 template <int CPR>
 __device__ __forceinline__ int pa_ksw(int r) { return CPR == 16 ? r & 15 : CPR == 8 ? (r >> 1) & 7 : (r >> 2) & 3; }
 
-// The same of V as bf16: a transposing read (16 rows, 32 bytes each) hits every
+// The same of V in 16 bits: a transposing read (16 rows, 32 bytes each) hits every
 // bank twice. The lowest bit lets neighbouring rows of e4m3, whose 16-byte pieces
 // become two chunks each, write to even and odd slots at once.
 template <int D>
@@ -155,7 +174,11 @@ struct PaTile {
   static constexpr int NB = KT / 16;            // 16-key blocks
   static constexpr int CPR = RB / 16;           // 16-byte chunks per row
   static constexpr int RPI = 64 / CPR;          // V rows per load instruction
-  static constexpr int LDS = KT * D * 2;        // one wave's slice: V as bf16, K (as it is) before it
+  static constexpr int LDS = KT * D * 2;        // one wave's slice: V in 16 bits, K (as it is) before it
+  typedef std::conditional_t<E4, f16x8_t, bf16x8_t> V8;  // the second product's operands
+  // A p is 2^kUp exp(s - m), in the sum too: fp16's smallest step is then 2^-38 of the
+  // largest p, so that many keys of little weight are not lost (2^-24 without it).
+  static constexpr float kUp = E4 ? 14.f : 0.f;
 };
 
 constexpr int kLineWaves = 8;
@@ -421,8 +444,8 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
         const int r = i * RPI + lr;
         if constexpr (E4) {
           const int at_ = ((2 * lc) ^ pa_sw<D>(r)) << 4;
-          *(bf16x8_t*)(sv + r * D * 2 + at_) = e4m3x8_to_bf16(vr[i][0], vr[i][1]);
-          *(bf16x8_t*)(sv + r * D * 2 + (at_ ^ 16)) = e4m3x8_to_bf16(vr[i][2], vr[i][3]);
+          *(f16x8_t*)(sv + r * D * 2 + at_) = e4m3x8_to_f16(vr[i][0], vr[i][1]);
+          *(f16x8_t*)(sv + r * D * 2 + (at_ ^ 16)) = e4m3x8_to_f16(vr[i][2], vr[i][3]);
         } else {
           *(pa_u32x4*)(sv + r * D * 2 + ((lc ^ pa_sw<D>(r)) << 4)) = vr[i];
         }
@@ -507,15 +530,24 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
       const float m_use = m_new == -INFINITY ? 0.f : m_new;
       const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
       m_run = m_new;
+      const float m_sub = m_use - T::kUp;
       float lsum = 0.f;
-      bf16x8_t pf[NB / 2];
+      typename T::V8 pf[NB / 2];
+      bf16x8_t pl[NB / 2];  // bf16: the halves that pf leaves over
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float e = __builtin_amdgcn_exp2f(s[b][r] - m_use);
+          const int i = 4 * (b & 1) + r;
+          const float e = __builtin_amdgcn_exp2f(s[b][r] - m_sub);
           lsum += e;
-          pf[b / 2][4 * (b & 1) + r] = (__bf16)e;
+          if constexpr (E4) {
+            pf[b / 2][i] = (_Float16)e;
+          } else {
+            const __bf16 h = (__bf16)e;
+            pf[b / 2][i] = h;
+            pl[b / 2][i] = (__bf16)(e - (float)h);
+          }
         }
       l_run = l_run * alpha + lsum;
 #pragma unroll
@@ -530,8 +562,14 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
           const pa_s16x4 vlo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pa_s16x4*)x);
           const pa_s16x4 vhi =
               __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pa_s16x4*)(x + 16 * D * 2));
-          const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(vlo, vhi, 0, 1, 2, 3, 4, 5, 6, 7));
-          oacc[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[b], oacc[db], 0, 0, 0);
+          const auto vf =
+              __builtin_bit_cast(typename T::V8, __builtin_shufflevector(vlo, vhi, 0, 1, 2, 3, 4, 5, 6, 7));
+          if constexpr (E4) {
+            oacc[db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[b], oacc[db], 0, 0, 0);
+          } else {
+            oacc[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[b], oacc[db], 0, 0, 0);
+            oacc[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pl[b], oacc[db], 0, 0, 0);
+          }
         }
     }
     if (step < steps) {
