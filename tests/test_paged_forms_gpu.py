@@ -1,4 +1,4 @@
-"""th_paged_attention in the forms that its cases take: the accuracy of the probabilities.
+"""The accuracy of th_paged_attention's probabilities and of th_paged_append's 8-bit stores.
 
 Bounds are elementwise, against 64 bits, in the terms of tests/test_paged_gpu.py: u(t) is a rounding's
 half step, A = sum_j p_j |v_j|, and a score is off by head_dim 2^-22 scale sum_i |q_i k_i| (an fp32 sum
@@ -102,3 +102,32 @@ def test_many_keys_of_little_weight_are_not_lost(gpu, cache, top, room):
         tol = tol + room * 2.0 ** -39 * 448.0
     assert (tol < 0.05 * ref).all()
     assert_within(out.view(1, 1, d), ref, tol)
+
+
+# ------------------------------------------------------------------ 8-bit stores
+@pytest.mark.parametrize("in_dtype", [BF16, torch.float32])
+@pytest.mark.parametrize("head_major", [False, True])   # head-major pages here are not whole pieces: one element a time
+def test_append_divides_by_the_scale(gpu, in_dtype, head_major):
+    """Halfway between two e4m3 values the quotient x / scale goes to the even one, bit for bit as torch's;
+    a product with the rounded reciprocal lands beside the middle."""
+    from torch_helion.hip import ops
+
+    announce(f"append, quotients halfway between two e4m3 values, {in_dtype} head_major={head_major}")
+    scales = torch.tensor([7.0, 3.0, 0.4375, 1.75, 5.0, 448.0, 1.0, 0.875])
+    hk, d = len(scales), 64
+    half = torch.cat([(torch.arange(17, 32, 2) / 16) * 2.0 ** e for e in range(-5, 11)])
+    half = torch.cat([half, -half]).view(-1, 1, d)                    # four tokens of 64 values
+    x = (half * scales[:, None]).to(BF16)                             # exact: five bits by at most three
+    ref = (x.float() / scales[:, None]).clamp(-448, 448).to(E4M3)
+    assert ((x.float() * (1 / scales[:, None])).clamp(-448, 448).to(E4M3).view(torch.uint8) != ref.view(torch.uint8)).sum() > 30
+    n = x.shape[0]
+    shape = (2, hk, 16, d + 3) if head_major else (2, 16, hk, d)
+    caches = [torch.zeros(shape, device=gpu).to(E4M3)[..., :d] for _ in range(2)]
+    if head_major:
+        caches = [c.transpose(1, 2) for c in caches]
+    rows = x.to(in_dtype).reshape(n, hk * d).to(gpu)
+    ops.paged_append(rows, rows, torch.arange(n, dtype=torch.int32, device=gpu), *caches,
+                     torch.tensor([[1]], dtype=torch.int32, device=gpu), rows=torch.zeros(n, dtype=torch.int32, device=gpu),
+                     k_scale=scales.to(gpu), v_scale=scales.to(gpu))
+    for c in caches:
+        assert torch.equal(c[1, :n].contiguous().view(torch.uint8).cpu(), ref.view(torch.uint8))
