@@ -7,6 +7,7 @@ tensor's device is missing.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 import subprocess
 from pathlib import Path
@@ -342,3 +343,60 @@ def test_page_book_refusals():
     for change, message in (({"device": "cpu"}, "HIP device"),):
         with pytest.raises(abi.HipBackendError, match=message):
             PagedKVCache(**{**sizes, **change})
+
+
+# ------------------------------------------------------------------ several devices
+class Devices:
+    """Stands for several devices: which one is current, and a library whose answers depend on it. As in the
+    library, th_init makes its device the current one."""
+
+    def __init__(self, monkeypatch):
+        from torch_helion.hip import abi, ops
+
+        self.current = 0
+        outer = self
+
+        class Guard:
+            def __init__(self, device):
+                self.to = device if isinstance(device, int) else torch.device(device).index
+
+            def __enter__(self):
+                self.was, outer.current = outer.current, self.to
+
+            def __exit__(self, *_):
+                outer.current = self.was
+
+        class Lib:
+            def th_paged_attention_workspace_bytes(self, *sizes):
+                return 1000 + outer.current
+
+        def init_device(device):
+            outer.current = device
+            return Lib()
+
+        monkeypatch.setattr(abi, "load", lambda path=None: Lib())
+        monkeypatch.setattr(abi, "init_device", init_device)
+        monkeypatch.setattr(torch.cuda, "device", Guard)
+        monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+        monkeypatch.setattr(torch.cuda, "current_device", lambda: self.current)
+        ops._paged_workspace.cache_clear()
+        monkeypatch.setattr(ops, "_paged_workspace", functools.lru_cache(maxsize=8)(ops._paged_workspace.__wrapped__))
+
+
+def test_workspace_is_asked_of_its_device(monkeypatch):
+    """The answer is the device's own, not the first one's, and the current device stays what it was."""
+    from torch_helion.hip import abi, ops
+
+    devices = Devices(monkeypatch)
+    for current in (0, 2, 0, 1):
+        devices.current = current
+        assert ops.paged_attention_workspace_bytes(4, 8, 2, 64, 4096) == 1000 + current
+        assert devices.current == current
+    for device in (1, "cuda:2", torch.device("cuda", 3), "cuda"):
+        devices.current = 0
+        index = 0 if device == "cuda" else torch.device("cuda", device).index if isinstance(device, int) else torch.device(device).index
+        assert ops.paged_attention_workspace_bytes(4, 8, 2, 64, 4096, device=device) == 1000 + index
+        assert devices.current == 0
+    with pytest.raises(abi.HipBackendError, match="HIP device"):
+        ops.paged_attention_workspace_bytes(4, 8, 2, 64, 4096, device="cpu")
+    assert ops._paged_workspace(5, 4, 8, 2, 64, 4096, 0, torch.bfloat16) == 1005 and devices.current == 0

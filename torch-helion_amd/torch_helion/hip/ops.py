@@ -8,6 +8,7 @@ library is missing or the device is not gfx950 they raise
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import functools
 import math
@@ -486,8 +487,10 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, k_ca
 @functools.lru_cache(maxsize=1024)
 def _paged_workspace(dev: int, tokens: int, heads_q: int, heads_kv: int, head_dim: int, max_keys: int, window: int,
                      dtype: torch.dtype) -> int:
-    lib = abi.load() if dev < 0 else abi.init_device(dev)
-    n = lib.th_paged_attention_workspace_bytes(tokens, heads_q, heads_kv, head_dim, th_dtype(dtype), max_keys, window)
+    # by the compute units of the current device: of dev, which th_init makes current, until here
+    with torch.cuda.device(dev) if dev >= 0 else contextlib.nullcontext():
+        lib = abi.init_device(dev) if dev >= 0 else abi.load()
+        n = lib.th_paged_attention_workspace_bytes(tokens, heads_q, heads_kv, head_dim, th_dtype(dtype), max_keys, window)
     if n < 0:
         _refuse("th_paged_attention_workspace_bytes", f"tokens={tokens} heads_q={heads_q} heads_kv={heads_kv} "
                                                       f"head_dim={head_dim} max_keys={max_keys} window={window} {dtype}")
@@ -495,10 +498,18 @@ def _paged_workspace(dev: int, tokens: int, heads_q: int, heads_kv: int, head_di
 
 
 def paged_attention_workspace_bytes(tokens: int, heads_q: int, heads_kv: int, head_dim: int, max_keys: int, *, window: int = 0,
-                                    dtype: torch.dtype = torch.bfloat16) -> int:
+                                    dtype: torch.dtype = torch.bfloat16, device: torch.device | str | int | None = None) -> int:
     """Workspace of :func:`paged_attention` over a cache of ``dtype`` whose page table has room for
-    ``max_keys`` keys a row (pages per row * page_size). 0 where it needs none."""
-    return _paged_workspace(-1, tokens, heads_q, heads_kv, head_dim, max_keys, window, dtype)
+    ``max_keys`` keys a row (pages per row * page_size), on ``device`` (the current one by default;
+    without any, that of an MI355X). 0 where it needs none."""
+    if device is None:
+        dev = torch.cuda.current_device() if torch.cuda.is_available() else -1
+    else:
+        at = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
+        if at.type != "cuda":
+            _refuse("th_paged_attention_workspace_bytes", f"device {device} is not a HIP device")
+        dev = torch.cuda.current_device() if at.index is None else at.index
+    return _paged_workspace(dev, tokens, heads_q, heads_kv, head_dim, max_keys, window, dtype)
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
