@@ -400,3 +400,44 @@ def test_workspace_is_asked_of_its_device(monkeypatch):
     with pytest.raises(abi.HipBackendError, match="HIP device"):
         ops.paged_attention_workspace_bytes(4, 8, 2, 64, 4096, device="cpu")
     assert ops._paged_workspace(5, 4, 8, 2, 64, 4096, 0, torch.bfloat16) == 1005 and devices.current == 0
+
+
+def test_paged_decode_block_on_another_device(monkeypatch):
+    """Built and stepped with its cache's device current, and the current one left as it was."""
+    from torch_helion.hip import decode, ops, paged
+
+    devices = Devices(monkeypatch)
+    seen = []
+    note = lambda *a, **k: seen.append(devices.current)
+
+    class Cache:
+        device = torch.device("cuda", 1)
+        k = torch.zeros(1, 4, 16, 2, 64)
+        page_table = torch.zeros(3, 4, dtype=torch.int32)
+        append = attend = staticmethod(note)
+
+    def build(self, state_dict, *, device, batch, **_):
+        note()
+        self.device, self.B, self.D, self.H, self.Hkv, self.hd, self.eps = device, batch, 256, 4, 2, 64, 1e-5
+        self.wqkv = self.g1 = self.q = self.attn = self.attn_ws = self.n_invalid = None
+        self.qkv = torch.zeros(batch, 8 * 64)
+
+    monkeypatch.setattr(decode.DecodeBlock, "__init__", build)
+    monkeypatch.setattr(decode.DecodeBlock, "_gemm", note)
+    monkeypatch.setattr(decode.DecodeBlock, "_after_attention", note)
+    blk = paged.PagedDecodeBlock({}, hidden=256, heads=4, kv_heads=2, intermediate=512, eps=1e-5, rope_theta=1e4, batch=3, cache=Cache())
+    x, pos = torch.zeros(3, 256, dtype=torch.bfloat16), torch.zeros(3, dtype=torch.int32)
+    blk.step(x, pos)
+    assert seen == [1] * 5 and devices.current == 0
+    devices.current = 1
+    blk.step(x, pos)
+    assert seen == [1] * 9 and devices.current == 1
+
+    asked = []
+    monkeypatch.setattr(ops, "paged_attention_workspace_bytes", lambda *a, device=None, **k: asked.append(device) or 0)
+    monkeypatch.setattr(torch, "empty", lambda *a, **k: None)
+    monkeypatch.setattr(torch, "zeros", lambda *a, **k: None)
+    blk.device, blk.max_len, blk.freqs = Cache.device, 64, Cache.k
+    monkeypatch.setattr(torch.Tensor, "to", lambda self, *a: self)
+    blk._allocate_cache()
+    assert asked == [Cache.device]

@@ -280,14 +280,15 @@ class PagedDecodeBlock(DecodeBlock):
         self.rope_scale, self.window, self.softcap = rope_scale, window, softcap
         self.freqs = ops.rope_frequencies(hidden // heads, rope_theta) if freqs is None else freqs
         max_len = cache.page_table.shape[1] * cache.k.shape[2]
-        super().__init__(state_dict, hidden=hidden, heads=heads, kv_heads=kv_heads, intermediate=intermediate, eps=eps,
-                         rope_theta=rope_theta, batch=batch, max_len=max_len, device=cache.device, fold_gain=fold_gain)
+        with torch.cuda.device(cache.device):
+            super().__init__(state_dict, hidden=hidden, heads=heads, kv_heads=kv_heads, intermediate=intermediate, eps=eps,
+                             rope_theta=rope_theta, batch=batch, max_len=max_len, device=cache.device, fold_gain=fold_gain)
 
     def _allocate_cache(self) -> None:
         self.freqs = self.freqs.to(self.device)
         self.qkv = torch.empty(self.B, (self.H + 2 * self.Hkv) * self.hd, device=self.device)
         n = ops.paged_attention_workspace_bytes(self.B, self.H, self.Hkv, self.hd, self.max_len, window=self.window,
-                                                dtype=self.cache.k.dtype)
+                                                dtype=self.cache.k.dtype, device=self.device)
         self.attn_ws = torch.empty(n, dtype=torch.uint8, device=self.device)
         self.n_invalid = torch.zeros(1, dtype=torch.int32, device=self.device)   # tokens that no page had room for
 
@@ -297,6 +298,9 @@ class PagedDecodeBlock(DecodeBlock):
         without is not stored and counted in ``self.n_invalid``). Returns the block output [batch, hidden] (bf16; ``self.out32`` holds it in fp32)."""
         if x.dtype != torch.bfloat16 or tuple(x.shape) != (self.B, self.D):
             _refuse("PagedDecodeBlock.step", "x must be bf16 [batch, hidden]")
+        if torch.cuda.current_device() != self.device.index:   # th_gemm launches on the current device
+            with torch.cuda.device(self.device):
+                return self.step(x, positions, rows)
         self._gemm(self.wqkv, x, [ops.EpiSpec(abi.EPI_ACC, self.qkv, a=0)], rscale_mask=0b1, lhs_gain=self.g1, sumsq=True,
                    inv_k=1.0 / self.D, eps=self.eps)
         qw, kvw = self.H * self.hd, self.Hkv * self.hd
