@@ -441,3 +441,19 @@ def test_paged_decode_block_on_another_device(monkeypatch):
     monkeypatch.setattr(torch.Tensor, "to", lambda self, *a: self)
     blk._allocate_cache()
     assert asked == [Cache.device]
+
+
+def test_attention_onto_its_queries_needs_their_stride(lib):
+    """With another stride a token's output would lie on queries that are still to be read; one token has none."""
+    from torch_helion.hip import abi
+
+    for tokens, ld_o, status in ((4, 512, abi.TH_ERR_INVALID), (4, 256, None), (1, 512, None)):
+        d = attn_desc(abi)
+        d.tokens, d.o, d.ld_o = tokens, d.q, ld_o
+        if status is None:
+            if torch.cuda.is_available():
+                continue
+            status = abi.TH_ERR_NOT_INIT
+        assert lib.th_paged_attention(C.byref(d), None) == status
+        if status == abi.TH_ERR_INVALID:
+            assert "in place" in abi.last_error(lib)

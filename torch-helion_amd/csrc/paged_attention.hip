@@ -808,6 +808,7 @@ extern "C" int th_paged_attention(const th_paged_attn_desc* d, void* stream) {
                (double)d->softcap);
   const int64_t row = (int64_t)d->heads_q * d->head_dim;
   TH_CHECK_ARG(d->ld_q >= row && d->ld_o >= row, "th_paged_attention: q/o row strides smaller than heads_q*head_dim");
+  TH_CHECK_ARG(d->q != d->o || d->ld_q == d->ld_o || d->tokens <= 1, "th_paged_attention: in place needs one row stride");
   const int per = d->cache_dtype == TH_BF16 ? 8 : 16;  // elements in 16 bytes
   TH_CHECK_ARG(d->k_stride_h >= d->head_dim && d->v_stride_h >= d->head_dim && d->k_stride_t >= d->head_dim &&
                    d->v_stride_t >= d->head_dim && d->k_stride_page >= d->head_dim && d->v_stride_page >= d->head_dim,
