@@ -293,9 +293,10 @@ int th_attention_decode(const th_decode_desc* desc, void* stream);
  *   a' = scale (a cos phi - b sin phi),  b' = scale (b cos phi + a sin phi),  phi = position * freqs[i]
  * pair i is dims (i, i + rot_dim/2), or (2i, 2i+1) with interleaved. Dims past
  * rot_dim are copied. inverse takes -phi: with the same scale that is the
- * gradient of the forward call. Angles are formed and reduced in 64 bits: off
- * by about |position * freqs[i]| 2^-53 radians, wherever the position lies. out
- * may be x itself (same row stride); otherwise the two must not overlap.
+ * gradient of the forward call. Angles are formed and reduced in 64 bits, the
+ * fraction of a turn that is left is an fp32: off by up to 3 |position *
+ * freqs[i]| 2^-53 + 1e-7 radians, and sine and cosine by two steps of 2^-24 more.
+ * out may be x itself (same row stride); otherwise the two must not overlap.
  */
 typedef struct th_rope_desc {
   int64_t tokens;

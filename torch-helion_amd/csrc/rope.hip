@@ -5,8 +5,9 @@
 // A pair (a, b) of a head at position p turns by phi = p f_i:
 //   a' = s (a cos phi - b sin phi),  b' = s (b cos phi + a sin phi).
 // Angles: p f_i / 2 pi is formed and reduced to a fraction of a turn in 64
-// bits (a float loses a whole turn's worth of it past a million positions) and
-// only the fraction goes through a single-precision sincospi. One token's
+// bits (at a million radians a float's step is 1/16 of one) and only the
+// fraction goes through a single-precision sincospi: 1e-7 radians from its
+// rounding to a float, and two steps of 2^-24 of the sine. One token's
 // angles serve all its heads, so a workgroup computes them once, into LDS.
 // Both kernels are HBM bound (three products per element read and written).
 #include "common.h"
