@@ -1,8 +1,11 @@
-"""The accuracy of th_paged_attention's probabilities and of th_paged_append's 8-bit stores.
+"""The paged entry points in the forms that their cases take: the accuracy of the attention's probabilities
+and of the 8-bit stores, batches over which the attention's waves take several tiles and tokens each, the
+inverse rotation by whole pieces, and the options of the cache and the block.
 
 Bounds are elementwise, against 64 bits, in the terms of tests/test_paged_gpu.py: u(t) is a rounding's
 half step, A = sum_j p_j |v_j|, and a score is off by head_dim 2^-22 scale sum_i |q_i k_i| (an fp32 sum
-in any order) and 2^-20 softcap; 2^-20 stands for the exponential.
+in any order), 2^-20 softcap and, with a bias, 2^-21 of the largest one (three roundings of it); 2^-20
+stands for the exponential. The fp32 sums over n keys are off by n 2^-23 of A.
 """
 
 from __future__ import annotations
@@ -11,7 +14,7 @@ import pytest
 import torch
 
 from conftest import announce
-from test_paged_gpu import BF16, E4M3, assert_within, gen, paged, u
+from test_paged_gpu import BF16, E4M3, ROT, assert_within, gen, paged, rope64, u
 
 pytestmark = pytest.mark.gpu
 
@@ -42,6 +45,7 @@ def attention64(q, kc, vc, table, pos, rows, scale, window=0, softcap=0.0, slope
         if softcap:
             s = softcap * torch.tanh(s / softcap)
         if slopes is not None:
+            err[i] += 2.0 ** -21 * slopes.to(dev).double().abs().view(h, 1) * (j[-1] - j[0] + 128)
             s = s - slopes.to(dev).double().view(hk, -1, 1) * (p - j).double()
         w = torch.softmax(s, -1)
         o[i], mag[i] = (w @ v).view(h, d), (w @ v.abs()).view(h, d)
@@ -104,6 +108,174 @@ def test_many_keys_of_little_weight_are_not_lost(gpu, cache, top, room):
     assert_within(out.view(1, 1, d), ref, tol)
 
 
+# ------------------------------------------------------------------ the line form
+def tiles_and_groups(gpu, lens, hq, hk, d, cache, window=0):
+    """(tiles of all tokens, groups of waves that they are dealt out to, keys of a tile) of the line form."""
+    keys = 8192 // (d * torch.empty(0, dtype=cache).element_size())
+    blocks = hk * -(-(hq // hk) // 16)
+    first = [max(0, n - window) // 16 * 16 if window else 0 for n in lens]
+    cus = torch.cuda.get_device_properties(gpu).multi_processor_count
+    return sum(-(-(n - a) // keys) for n, a in zip(lens, first) if n > 0), cus * 8 // blocks, keys
+
+
+def check_line(gpu, lens, hq, hk, d, cache, *, room, rows=None, window=0, softcap=0.0, slopes=False, amplitude=1.0, least=2.0, seed=0,
+               ps=16):
+    """A call in the line form with at least ``least`` tiles for each group of waves, against 64 bits; NaN in every
+    slot that no token sees and in the workspace; a second call gives the same bits."""
+    from torch_helion.hip import ops
+
+    tiles, groups, _ = tiles_and_groups(gpu, lens, hq, hk, d, cache, window)
+    assert tiles >= least * groups, (tiles, groups)
+    g = gen(seed + 31 * d + hq)
+    t, n_rows = len(lens), (len(lens) if rows is None else max(rows) + 1)
+    kc, vc, table = paged(n_rows, room // ps, ps, hk, d, cache, g, gpu)
+    pos = torch.tensor(lens, dtype=torch.int32) - 1
+    rt = None if rows is None else torch.tensor(rows, dtype=torch.int32)
+    seen = torch.zeros(kc.shape[:2], dtype=torch.bool, device=gpu)
+    for i, n in enumerate(lens):
+        j = torch.arange(max(0, n - window) if window else 0, max(n, 0), device=gpu)
+        seen[table[i if rows is None else rows[i]].long()[j // ps], j % ps] = True
+    for c in (kc, vc):
+        c.copy_(torch.where(seen[:, :, None, None], c.float(), float("nan")).to(cache))
+    table = torch.where(seen.any(1)[table.long()], table, torch.full_like(table, -1))
+    q = (torch.randn(t, hq * d, generator=g) * amplitude).to(BF16)
+    sl = torch.rand(hq, generator=g) * 0.1 if slopes else None
+    sc = {n: (torch.rand(hk, generator=g) + 0.5).to(gpu) for n in ("k_scale", "v_scale")} if cache == E4M3 else {}
+    size = ops.paged_attention_workspace_bytes(t, hq, hk, d, room, window=window, dtype=cache, device=gpu)
+    assert size > 0                                                  # the line form: the pair form needs none
+    outs = []
+    for _ in range(2):
+        out = torch.full((t, hq * d), float("nan"), dtype=BF16, device=gpu)
+        ops.paged_attention(q.to(gpu), kc, vc, table, pos.to(gpu), out, scale=d ** -0.5, rows=None if rt is None else rt.to(gpu),
+                            window=window, softcap=softcap, slopes=None if sl is None else sl.to(gpu),
+                            workspace=torch.full((size,), 255, dtype=torch.uint8, device=gpu), **sc)
+        outs.append(out)
+    torch.cuda.synchronize()
+    assert torch.equal(*outs)
+    ref, mag, err = attention64(q.view(t, hq, d), kc, vc, table, pos, rt, d ** -0.5, window, softcap, sl, sc.get("k_scale"), sc.get("v_scale"))
+    most = max(lens)
+    tol = u(BF16) * ref.abs() + mag * (1 + u(BF16)) * (2 * err + p_step(cache) + most * 2.0 ** -23) + 1e-30
+    if cache == E4M3:
+        tol = tol + most * 2.0 ** -39 * 448.0
+    assert_within(outs[0].view(t, hq, d), ref, tol)
+    empty = [i for i, n in enumerate(lens) if n <= 0]
+    assert (outs[0][empty] == 0).all()
+
+
+@pytest.mark.parametrize("group", [1, 3, 4, 8, 16, 20])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+def test_line_of_cut_tokens(gpu, cache, d, group):
+    """320 pairs of ragged lengths over 64 groups: waves go from token to token, past empty ones, and the parts of
+    cut tokens are joined by workgroups of several heads (8 heads of 128 dims at most, a second block of 4 heads at
+    group 20, rows that no head takes at group 3)."""
+    announce(f"paged attention, cut tokens, {cache} d={d} group={group}")
+    keys = tiles_and_groups(gpu, [], 1, 1, d, cache)[2]
+    lens = [0, int(40.3 * keys), 1, int(30.9 * keys), 0, int(60.5 * keys), 17 * keys, 33 * keys + 1, 25 * keys - 1, 0]
+    check_line(gpu, lens, 32 * group, 32, d, cache, room=64 * keys, least=3)
+
+
+@pytest.mark.parametrize("lens,hq,hk,d,cache,room", [
+    ([100003, 17], 8, 2, 128, BF16, 100016),               # few heads: the join by 32 dims
+    ([70001], 4, 1, 64, E4M3, 70016), ([0, 150000, 0], 3, 1, 64, BF16, 150000),
+    ([3000, 2999, 2047, 0, 4000, 2500], 64, 8, 128, BF16, 4096),   # fewer than 256 pairs: a head a workgroup
+    ([9000, 5000, 0, 7001], 48, 16, 64, E4M3, 9008),
+])
+def test_line_of_few_tokens(gpu, lens, hq, hk, d, cache, room):
+    announce(f"paged attention, few tokens, lens={lens} hq={hq} hk={hk} d={d} {cache}")
+    check_line(gpu, lens, hq, hk, d, cache, room=room, least=0.2)
+
+
+@pytest.mark.parametrize("d,cache", [(64, BF16), (128, BF16), (64, E4M3), (128, E4M3)])
+def test_line_cut_at_its_tokens_ends(gpu, d, cache):
+    """Stretches that end where tokens end: 32 tokens of four tiles for 32 groups (each finished by its group), 16 of
+    eight (each two whole stretches), and the same with one tile more at the front (every cut moves by a little)."""
+    announce(f"paged attention, even stretches, d={d} {cache}")
+    _, groups, keys = tiles_and_groups(gpu, [], 64, 64, d, cache)
+    for lens in ([4 * keys] * groups, [8 * keys] * (groups // 2), [1] + [4 * keys] * groups, [keys] + [0, 8 * keys] * (groups // 2)):
+        check_line(gpu, lens, 64, 64, d, cache, room=33 * keys, rows=[i % 3 for i in range(len(lens))], least=4)
+
+
+@pytest.mark.parametrize("window,softcap,slopes,d,cache,hq,hk", [
+    (1500, 0.0, False, 128, BF16, 128, 32), (2500, 20.0, True, 64, BF16, 96, 32), (4400, 0.0, True, 64, E4M3, 64, 32),
+    (2300, 5.0, False, 128, E4M3, 128, 32), (0, 30.0, True, 128, BF16, 32, 32), (0, 8.0, False, 64, E4M3, 160, 32),
+    (0, 0.0, True, 128, E4M3, 64, 16), (1100, 1.0, True, 128, BF16, 640, 32),
+])
+def test_line_with_window_cap_and_bias(gpu, window, softcap, slopes, d, cache, hq, hk):
+    announce(f"paged attention, line, window={window} softcap={softcap} slopes={slopes} d={d} {cache} hq={hq}")
+    keys = tiles_and_groups(gpu, [], 1, 1, d, cache)[2]
+    top = 80 * keys
+    w = window or top // 2
+    lens = [0, top, w - 1, w, w + 1, 0, w + 16, 1, top - 15, 3 * w // 2, 0, 0, top // 3, top - 1]
+    check_line(gpu, lens, hq, hk, d, cache, room=top, window=window, softcap=softcap, slopes=slopes, amplitude=4.0)
+
+
+@pytest.mark.parametrize("tokens,hq,hk,d,cache,top", [
+    (513, 8, 4, 64, BF16, 2200), (1300, 2, 1, 64, BF16, 3000), (1024, 6, 2, 128, E4M3, 1500), (1500, 4, 4, 128, BF16, 900),
+    (600, 20, 1, 64, E4M3, 5000),
+])
+def test_line_of_many_tokens(gpu, tokens, hq, hk, d, cache, top):
+    """More than 512 tokens (several of them to a thread that counts their tiles), with empty ones at the front, at
+    the end, at both ends of such runs and whole runs of them; seven rows hold the keys."""
+    announce(f"paged attention, {tokens} tokens, hq={hq} hk={hk} d={d} {cache}")
+    keys = tiles_and_groups(gpu, [], 1, 1, d, cache)[2]
+    run = -(-tokens // 512)
+    lens = [1 + (i * 7919) % top for i in range(tokens)]
+    for i in range(tokens):
+        if i < 11 or i >= tokens - 5 or i % (5 * run) == 0 or i % (7 * run) == run - 1 or 40 * run <= i < 47 * run:
+            lens[i] = 0
+    check_line(gpu, lens, hq, hk, d, cache, room=-(-max(top, 33 * keys) // 64) * 64, rows=[i % 7 for i in range(tokens)], ps=64)
+
+
+@pytest.mark.parametrize("tokens,hk", [(700, 1), (1200, 8)])
+def test_line_of_many_short_tokens(gpu, tokens, hk):
+    """More than 512 tokens of a tile at most, most of them empty: fewer tiles than waves."""
+    announce(f"paged attention, {tokens} short tokens of {hk} kv heads")
+    lens = [(1 + i % 60) * (i % 17 == 3) for i in range(tokens)]
+    tiles, groups, _ = tiles_and_groups(gpu, lens, 2 * hk, hk, 64, BF16)
+    assert tiles < groups
+    check_line(gpu, lens, 2 * hk, hk, 64, BF16, room=4096, rows=[i % 5 for i in range(tokens)], least=0)
+
+
+# ------------------------------------------------------------------ the inverse rotation
+@pytest.mark.parametrize("t,h,d,rot,interleaved,dtype,idx", [
+    (70, 32, 128, 128, False, BF16, torch.int32), (33, 8, 128, 64, True, BF16, torch.int64), (129, 4, 64, 64, False, torch.float32, torch.int32),
+    (16, 12, 128, 128, True, torch.float32, torch.int64), (17, 3, 128, 104, False, BF16, torch.int32), (9, 5, 64, 40, True, BF16, torch.int32),
+])
+def test_rope_inverse_by_whole_pieces(gpu, t, h, d, rot, interleaved, dtype, idx):
+    """The first four have rows and rotated halves in whole 16-byte pieces, the last two go element by element:
+    the gradient is the transpose of the formula's matrix, and turning there and back gives scale^2 x."""
+    from torch_helion.hip import ops
+
+    announce(f"rope inverse t={t} h={h} d={d} rot={rot} interleaved={interleaved} {dtype}")
+    g = gen(t + rot)
+    go = torch.randn(t, h * d, generator=g).to(dtype)
+    pos = torch.randint(0, 5000, (t,), generator=g, dtype=idx)
+    f = ops.rope_frequencies(rot, 10000.0)
+    x = torch.zeros(t, h, d, dtype=torch.float64, requires_grad=True)
+    n = rot // 2
+    ia = torch.arange(n) * (2 if interleaved else 1)
+    ib = ia + (1 if interleaved else n)
+    ang = pos.double()[:, None, None] * f
+    a, b = x[..., ia], x[..., ib]
+    ga, gb = go.double().view(t, h, d)[..., ia], go.double().view(t, h, d)[..., ib]
+    turned = ((a * ang.cos() - b * ang.sin()) * ga + (b * ang.cos() + a * ang.sin()) * gb).sum() * 1.25
+    (ref,) = torch.autograd.grad(turned + (x[..., rot:] * go.double().view(t, h, d)[..., rot:]).sum(), x)
+    _, mag = rope64(go.view(t, h, d), pos, f, interleaved, 1.25, inverse=True)
+    half = u(dtype) if dtype == BF16 else 0.0
+    got = torch.full((t, h * d), float("nan"), dtype=dtype, device=gpu)
+    kw = dict(head_dim=d, interleaved=interleaved, scale=1.25)
+    ops.rope(go.to(gpu), pos.to(gpu), f.to(gpu), got, inverse=True, **kw)
+    assert_within(got.view(t, h, d), ref, ROT * mag + half * ref.abs() + 1e-30)
+    there, back = torch.empty_like(got), torch.empty_like(got)
+    ops.rope(go.to(gpu), pos.to(gpu), f.to(gpu), there, **kw)
+    ops.rope(there, pos.to(gpu), f.to(gpu), back, inverse=True, **kw)
+    want = go.double().view(t, h, d).clone()
+    want[..., :rot] *= 1.25 ** 2
+    # the first turn's roundings, turned back and scaled, then the second's own
+    assert_within(back.view(t, h, d), want, (2 * ROT + 2 * half) * 1.25 * 2 * mag + half * want.abs() + 1e-30)
+
+
 # ------------------------------------------------------------------ 8-bit stores
 @pytest.mark.parametrize("in_dtype", [BF16, torch.float32])
 @pytest.mark.parametrize("head_major", [False, True])   # head-major pages here are not whole pieces: one element a time
@@ -131,3 +303,67 @@ def test_append_divides_by_the_scale(gpu, in_dtype, head_major):
                      k_scale=scales.to(gpu), v_scale=scales.to(gpu))
     for c in caches:
         assert torch.equal(c[1, :n].contiguous().view(torch.uint8).cpu(), ref.view(torch.uint8))
+
+
+# ------------------------------------------------------------------ options of the cache and the block
+@pytest.mark.parametrize("cache_type,options", [
+    (BF16, dict(window=20, softcap=4.0)), (BF16, dict(rope_scale=1.2)), (E4M3, dict(window=33, rope_scale=0.9, softcap=15.0)),
+    (E4M3, {}),
+])
+def test_block_options_and_scaled_pages(gpu, cache_type, options):
+    """A step of the block with a window, a cap, a scaled rotation of frequencies of its own and, for an e4m3 cache,
+    scales: what it stores and attends against 64 bits from its own projections; a captured step gives its bits."""
+    from targets.llama_block import LlamaBlockConfig
+    from test_e2e_gpu import _decode_case
+    from torch_helion.hip import ops
+    from torch_helion.hip.paged import PagedDecodeBlock, PagedKVCache
+
+    announce(f"paged block {cache_type} {options}")
+    cfg = LlamaBlockConfig(batch=5, seq=80, causal=True, dtype=BF16, rope_theta=500000.0, hidden=256, heads=4, kv_heads=2, intermediate=512)
+    sd, x, *_ = _decode_case(cfg, cfg.seq, seed=4)
+    hk, d, layer = cfg.n_kv, cfg.head_dim, 1
+    g = gen(6)
+    sc = {n: torch.rand(2, hk, generator=g) * 0.02 + 0.01 for n in ("k_scale", "v_scale")} if cache_type == E4M3 else {}
+    cache = PagedKVCache(layers=2, pages=40, page_size=16, kv_heads=hk, head_dim=d, rows=6, max_len=128, dtype=cache_type, device=gpu, **sc)
+    freqs = ops.rope_frequencies(d - 16, 10000.0, scaling="linear", factor=2.0)
+    blk = PagedDecodeBlock(sd, hidden=cfg.hidden, heads=cfg.heads, kv_heads=hk, intermediate=cfg.intermediate, eps=cfg.eps,
+                           rope_theta=cfg.rope_theta, batch=cfg.batch, cache=cache, layer=layer, freqs=freqs, **options)
+    pos = [70, 0, -1, 31, 100]
+    rows = [cache.open() for _ in range(5)]
+    for r, p in zip(rows, pos):
+        if p >= 0:
+            cache.extend({r: p + 1})
+            kv = [torch.randn(p + 1, hk * d, generator=g).to(BF16).to(gpu) for _ in range(2)]
+            cache.append(layer, *kv, torch.arange(p + 1, dtype=torch.int32, device=gpu),
+                         rows=torch.full((p + 1,), r, dtype=torch.int32, device=gpu))
+    pt, rt = (torch.tensor(a, dtype=torch.int32, device=gpu) for a in (pos, rows))
+    xs = x.to(gpu)
+    blk.step(xs, pt, rt)
+    torch.cuda.synchronize()
+    q, k, v = (a.reshape(5, -1, d) for a in blk.qkv.cpu().split([cfg.heads * d, hk * d, hk * d], 1))
+    scale = options.get("rope_scale", 1.0)
+    live = [i for i, p in enumerate(pos) if p >= 0]
+    at = pt.cpu()[live]
+    (rq, mq), (rk, mk) = (rope64(a[live], at, freqs, False, scale) for a in (q, k))
+    assert_within(blk.q.view(5, -1, d)[live], rq, ROT * mq + u(BF16) * rq.abs() + 1e-30, "q")
+    page = torch.tensor([cache.book.pages[rows[i]][pos[i] // 16] for i in live])
+    for pages, ref, mag, name in ((cache.k, rk, mk, "k_scale"), (cache.v, v[live].double(), torch.zeros_like(rk), "v_scale")):
+        tol = ROT * mag + u(BF16) * ref.abs() + 1e-30
+        if cache_type == E4M3:
+            s = sc[name][layer].double()[:, None]
+            ref, mag = (ref / s).clamp(-448, 448), mag / s
+            tol = (ROT * mag + 2.0 ** -23 * ref.abs()) * (1 + u(E4M3)) + torch.clamp(u(E4M3) * ref.abs(), min=2.0 ** -10)
+        assert_within(pages[layer].float().cpu()[page, at.long() % 16], ref, tol, name)
+    mine = {n: s[layer].to(gpu) for n, s in sc.items()}
+    ref, mag, err = attention64(blk.q.view(5, -1, d), cache.k[layer], cache.v[layer], cache.page_table, pt, rt, d ** -0.5,
+                                options.get("window", 0), options.get("softcap", 0.0), None, mine.get("k_scale"), mine.get("v_scale"))
+    tol = u(BF16) * ref.abs() + mag * (1 + u(BF16)) * (2 * err + p_step(cache_type) + 128 * 2.0 ** -23) + 1e-30
+    assert_within(blk.attn.view(5, -1, d), ref, tol, "attention")
+    assert blk.n_invalid.item() == 0 and torch.isfinite(blk.out32).all()
+    want = [t.clone() for t in (blk.out32, cache.k.view(torch.uint8), cache.v.view(torch.uint8))]
+    blk.capture(xs, pt, rt)
+    for _ in range(3):
+        blk.out32.zero_()
+        blk.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip((blk.out32, cache.k.view(torch.uint8), cache.v.view(torch.uint8)), want))
