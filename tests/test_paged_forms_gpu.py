@@ -108,6 +108,35 @@ def test_many_keys_of_little_weight_are_not_lost(gpu, cache, top, room):
     assert_within(out.view(1, 1, d), ref, tol)
 
 
+@pytest.mark.parametrize("room", [64, 8192])
+@pytest.mark.parametrize("cache", [BF16, E4M3])
+@pytest.mark.parametrize("top", [2.0 ** e for e in (20, 24, 25, 26, 27, 28, 29, 40, 100)])
+def test_scores_whose_steps_are_large(gpu, cache, top, room):
+    """The largest score at top and at 1.5 top, the others a few steps of an fp32 of that size below it or far
+    away: an exact score (one product of powers of two) leaves weight 1, split evenly, on the keys that have it."""
+    from torch_helion.hip import ops
+
+    announce(f"paged attention, scores of {top}, {cache} room={room}")
+    d, ps, n = 64, 16, 60
+    kc = torch.zeros(room // ps, ps, 2, d, device=gpu)
+    at = torch.tensor([1.0, -1.0, 0.5, 0.0, 0.875, 1.0])
+    for j in range(n):
+        kc[j // ps, j % ps, :, 0] = at[j % 6]
+    vc = torch.randn(room // ps, ps, 2, d, generator=gen(int(top) % 97)).to(gpu).to(cache)
+    kc = kc.to(cache)
+    table = torch.arange(room // ps, dtype=torch.int32, device=gpu)[None]
+    q = torch.zeros(1, 4, d)
+    q[0, :, 0] = torch.tensor([top, 1.5 * top, -top, -1.5 * top])
+    pos = torch.tensor([n - 1], dtype=torch.int32, device=gpu)
+    out = torch.empty(1, 4 * d, dtype=BF16, device=gpu)
+    ops.paged_attention(q.view(1, -1).to(BF16).to(gpu), kc, vc, table, pos, out, scale=1.0)
+    torch.cuda.synchronize()
+    best = [[j for j in range(n) if at[j % 6] == (1.0 if h < 2 else -1.0)] for h in range(4)]
+    ref = torch.stack([torch.stack([vc[j // ps, j % ps, h // 2].double().cpu() for j in js]).mean(0) for h, js in enumerate(best)])
+    mag = torch.stack([torch.stack([vc[j // ps, j % ps, h // 2].double().cpu().abs() for j in js]).mean(0) for h, js in enumerate(best)])
+    assert_within(out.view(4, d), ref, u(BF16) * ref.abs() + mag * (1 + u(BF16)) * n * 2.0 ** -23 + 1e-30)
+
+
 # ------------------------------------------------------------------ the line form
 def tiles_and_groups(gpu, lens, hq, hk, d, cache, window=0):
     """(tiles of all tokens, groups of waves that they are dealt out to, keys of a tile) of the line form."""

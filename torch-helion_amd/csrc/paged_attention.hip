@@ -176,9 +176,12 @@ struct PaTile {
   static constexpr int RPI = 64 / CPR;          // V rows per load instruction
   static constexpr int LDS = KT * D * 2;        // one wave's slice: V in 16 bits, K (as it is) before it
   typedef std::conditional_t<E4, f16x8_t, bf16x8_t> V8;  // the second product's operands
-  // A p is 2^kUp exp(s - m), in the sum too: fp16's smallest step is then 2^-38 of the
-  // largest p, so that many keys of little weight are not lost (2^-24 without it).
-  static constexpr float kUp = E4 ? 14.f : 0.f;
+  // What the exponents of a softmax with maximum m are taken from, and its parts joined by.
+  // For fp16 14 less, so that its smallest step is 2^-38 of the largest p and many keys of
+  // little weight are not lost (2^-24 with m itself). From 2^24 on a float's own steps are
+  // 2 and more, and m - 14 could round to m - 16, of which a p overflows: there it is m.
+  // (A product with 2^14 after the exponential: 97.3 us for 95.5, 64 rows of 1-8191 keys.)
+  static __device__ __forceinline__ float from(float m) { return E4 && fabsf(m) < 0x1p24f ? m - 14.f : m; }
 };
 
 constexpr int kLineWaves = 8;
@@ -399,7 +402,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
 
   bf16x8_t qf[NKS];
   f32x4_t oacc[NDB];
-  float m_run = 0.f, l_run = 0.f, mul = 0.f, slope = 0.f;
+  float m_run = 0.f, r_run = 0.f, l_run = 0.f, mul = 0.f, slope = 0.f;
   // capped: softcap log2(e) tanh(mul s / (2 log2(e))), else mul s
   const bool cap = p.softcap > 0.f;
   const float mul0 = p.scale * (cap ? 2.f * kLog2e / p.softcap : kLog2e);
@@ -423,7 +426,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
       for (int d = 0; d < NDB; ++d)
 #pragma unroll
         for (int r = 0; r < 4; ++r) oacc[d][r] = 0.f;
-      m_run = -INFINITY;
+      m_run = r_run = -INFINITY;
       l_run = 0.f;
       mul = mul0 * kscale_n;
       slope = slope_n * kLog2e;
@@ -527,10 +530,10 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
       mloc = fmaxf(mloc, __shfl_xor(mloc, 16));
       mloc = fmaxf(mloc, __shfl_xor(mloc, 32));
       const float m_new = fmaxf(m_run, mloc);
-      const float m_use = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = __builtin_amdgcn_exp2f(m_run - m_use);
+      const float r_new = T::from(m_new), r_use = m_new == -INFINITY ? 0.f : r_new;
+      const float alpha = __builtin_amdgcn_exp2f(r_run - r_use);
       m_run = m_new;
-      const float m_sub = m_use - T::kUp;
+      r_run = r_new;
       float lsum = 0.f;
       typename T::V8 pf[NB / 2];
       bf16x8_t pl[NB / 2];  // bf16: the halves that pf leaves over
@@ -539,7 +542,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int i = 4 * (b & 1) + r;
-          const float e = __builtin_amdgcn_exp2f(s[b][r] - m_sub);
+          const float e = __builtin_amdgcn_exp2f(s[b][r] - r_use);
           lsum += e;
           if constexpr (E4) {
             pf[b / 2][i] = (_Float16)e;
@@ -600,7 +603,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
       lds_barrier();  // every wave is done with its V tile
       if (qc < gn) {
         if (g == 0) {
-          mw[wave][qc] = m_run;
+          mw[wave][qc] = r_run;
           lw[wave][qc] = l;
         }
 #pragma unroll
@@ -632,7 +635,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
       } else {
         const int64_t slot = (int64_t)(2 * me + (u_begin != u0)) * p.gq + qc;
         if (g == 0) {
-          p.ml[2 * slot] = m_run;
+          p.ml[2 * slot] = r_run;
           p.ml[2 * slot + 1] = l;
         }
 #pragma unroll
