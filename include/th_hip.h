@@ -369,8 +369,10 @@ int th_paged_append(const th_paged_append_desc* desc, void* stream);
  * key (padded, or of a row outside the table) gets zeros. What the slots of
  * unseen keys hold, NaN included, does not reach the result. The keys of all
  * tokens are dealt out evenly over the GPU, whatever the lengths, and the
- * parts are joined through the workspace (which short rows do not need). o may
- * be q (same row stride).
+ * parts are joined through the workspace (which short rows do not need). Sums
+ * and maxima are fp32; a softmax's numerators meet the values off by 2^-16 over a
+ * bf16 cache, by 2^-11 (or 2^-39 of the largest) over an e4m3 one. o may be q
+ * (same row stride).
  */
 typedef struct th_paged_attn_desc {
   int32_t tokens, heads_q, heads_kv, head_dim;  /* tokens <= 65535, head_dim 64 or 128 */

@@ -25,7 +25,7 @@
 //            only a few tiles by its table and window, one launch and no line to
 //            lay out.
 //
-// One tile:
+// One tile (figures of alternatives were taken with p as one bf16 half, 0.6 us less):
 //   V        loaded by whole rows (16-byte pieces, consecutive lanes next to each
 //            other) and staged in 16 bits in the wave's own LDS slice, swizzled.
 //   S^T      = K Q^T, v_mfma_f32_16x16x32_bf16: lane l supplies row l % 16 and 8
@@ -195,11 +195,11 @@ __device__ __forceinline__ void keep_step(int64_t step) {
 
 // NW: waves of a workgroup. NT: what is loaded past the caches (non-temporal): 1 V,
 // 2 a bf16 K too. In a graph, us, with neither, V, both: 64 sequences of 2048-4096
-// keys 149.4, 136.1, 132.1, two of 100-131k 176, 161, 157; an 8-bit cache 105.4
-// without and 97.3 with (its K, in half lines, past the caches too: 107). Where
-// what is read stays in the 256 MB last-level cache it costs: 288 windows of 1000
-// (pair form) 17.0, 19.5, 20.1, 64 short lines (82 MB) 25.2, 26.3, 27.6; caches of
-// that size that are not there yet, 16 sequences of 500-4000 keys: 40.2, 37.2, 37.9.
+// keys 149.7, 136.9, 132.9, two of 100-131k 171.5, 155.4, 152.2; an 8-bit cache, 64
+// of 1-8191, 100.5, 92.3, 93.6. Where what is read stays in the 256 MB last-level
+// cache it costs: 288 windows of 1000 (pair form) 17.6, 19.7, 19.9, 64 short lines
+// (82 MB) 25.2, 26.3, 27.6; caches of that size that are not there yet, 16 sequences
+// of 500-4000 keys: 40.2, 37.2, 37.9.
 template <int D, bool E4, bool PAIR, int NW, int NT>
 __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2, 2))) paged_attn_kernel(PAttnK p) {
   using T = PaTile<D, E4>;
@@ -753,13 +753,14 @@ static int64_t most_tiles(int64_t max_keys, int window, int row_bytes) {
 }
 
 // Whether pairs take the pair form. In a graph, us, pair against line form, lengths
-// of half to all of the room (bf16, 128 dims, 8 kv heads, 4 query heads each):
+// of half to all of the room, one token all of it (bf16, 128 dims, 8 kv heads, 4
+// query heads each):
 //   tiles of room      16            32            64
-//     8 pairs       6.4 /  8.9    7.9 /  9.0   11.1 /  9.3
-//   128 pairs       9.8 / 14.5   14.7 / 20.6   23.5 / 28.0
-//   512 pairs      20.5 / 28.6   39.0 / 43.1   75.9 / 76.8
-//  2048 pairs      69.0 / 80.7    130 /  142    255 /  259
-// and with an e4m3 cache at 32 tiles 10.5 / 9.5 for 8 pairs, 18.4 / 22.3 for 128.
+//     8 pairs       8.3 /  9.2   11.5 /  9.4   19.1 / 10.3
+//   128 pairs      10.1 / 14.3   15.2 / 20.8   24.0 / 28.3
+//   512 pairs      20.8 / 28.7   38.2 / 44.0   73.3 / 74.9
+//  2048 pairs      69.8 / 81.2    130 /  141    255 /  259
+// and with an e4m3 cache at 32 tiles 16.4 / 9.8 for 8 pairs, 18.5 / 22.0 for 128.
 // 64 tiles and more stay with the line: lengths are not known here, and one full
 // row among short ones would cost the pair form 20 us where the line takes 9.
 static bool pair_form(int64_t tiles, int64_t pairs) { return tiles <= 16 || (tiles <= 32 && pairs >= 128); }
@@ -767,11 +768,11 @@ static bool pair_form(int64_t tiles, int64_t pairs) { return tiles <= 16 || (til
 // Waves of a pair's workgroup: as many as the pair can have tiles, while the CUs
 // (eight waves each) hold all pairs at once. us with 4, 2, 1 waves, bf16, 128 dims:
 //   tiles of room          1                  2                   4                   8
-//   512 pairs       5.9  5.3  5.1      6.1  5.7  6.5      8.8  9.0 10.4     12.3 13.3 16.7
-//   768 pairs       9.0  5.6  5.3      9.8  7.1  8.0     12.9 10.8 12.3     17.9 16.2 18.9
-//  2048 pairs      18.6 12.6  8.9     19.8 15.1 13.0     23.9 21.9 20.2     40.8 42.8 41.3
+//   512 pairs       6.0  5.5  5.2      6.4  5.9  6.6      9.1  9.1 10.9     12.7 13.8 17.5
+//   768 pairs       9.2  5.8  5.4     10.0  7.4  8.0     13.0 11.2 12.6     18.3 16.7 19.6
+//  2048 pairs      18.9 12.9  9.2     20.3 15.5 13.5     24.5 22.6 21.4     41.6 44.9 37.1
 // Past 8 tiles 8 waves where there is a CU for each pair (256 pairs, 16 tiles of
-// e4m3: 16.1 against 16.7 with 4, 32 tiles 24.1 against 27.5), else 4.
+// e4m3: 15.9 against 17.0 with 4, 32 tiles 24.6 against 26.8), else 4.
 static int pair_waves(int64_t tiles, int64_t pairs) {
   const int64_t cus = line_grid();
   if (tiles > 8) return pairs <= cus ? 8 : 4;
@@ -870,9 +871,9 @@ extern "C" int th_paged_attention(const th_paged_attn_desc* d, void* stream) {
     // Heads of a token side by side on one XCD, whose L2 they share: where a row is half
     // a 128-byte line (the other half is the next head's), and from 512 MB on, where
     // neighbours are read together. us, in order and so: 64-byte rows of 512 pairs, 16
-    // tiles 37.7 / 26.7, of 5600 pairs, 32 tiles 683 / 476; 128-byte rows of 2048 pairs,
-    // 32 tiles 152 / 142, of 5600 pairs 389 / 342; 256-byte rows 134 / 135, 353 / 347;
-    // smaller calls lose 2 to 5 percent: 512 pairs, 16 tiles 21.7 / 23.3.
+    // tiles 36.8 / 27.0, of 5600 pairs, 32 tiles 679 / 477; 128-byte rows of 2048 pairs,
+    // 32 tiles 152 / 143, of 5600 pairs 388 / 341; 256-byte rows 134 / 135, 351 / 346;
+    // smaller calls lose up to 5 percent: 512 pairs, 16 tiles 21.1 / 21.4.
     k.turn = d->head_dim * es < 128 || pairs * tiles >= (512 << 20) / 16384 ? 8 * d->heads_kv * k.nqb : 0;
     launch_paged(k, d->head_dim, e4, pair_waves(tiles, pairs), pairs * tiles > (128 << 20) / 16384, (unsigned)pairs, s);
     TH_CHECK_LAUNCH();

@@ -367,7 +367,7 @@ static void launch_rope(const RopeK& k, int64_t tokens, hipStream_t s) {
   // More than half of the 256 MB last-level cache would not be there for the next
   // kernel anyway. 16384 x 32 x 128 bf16 (268 MB) 47.8 -> 44.7 us, with its stores
   // past the caches too 47.3; 16004 prompt tokens into an e4m3 cache (361 MB) 71.3 ->
-  // 67.5, with the loads alone 74.8.
+  // 67.5, with the loads alone 74.8 (1.4 us more each since the scale divides).
   const int64_t bytes = tokens * (((int64_t)k.hq + 2 * k.hkv) * k.hd * (int)sizeof(InT) + (int64_t)k.hq * k.hd * (int)sizeof(OutT) +
                                   2 * (int64_t)k.hkv * k.hd * (int)sizeof(CacheT));
   const dim3 grid = grid_of(cdiv(tokens, tpb));

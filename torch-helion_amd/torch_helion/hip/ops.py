@@ -389,8 +389,9 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, out: tor
 
     Pairs are dims (i, i + len(freqs)), or (2 i, 2 i + 1) with ``interleaved``; ``scale`` multiplies
     the rotated dims, the others are copied. ``inverse`` turns back: called on the gradient of the
-    output with the same scale it gives the gradient of x. ``out`` may be x; otherwise the two must
-    not overlap."""
+    output with the same scale it gives the gradient of x. Like every call here it writes into
+    ``out`` and records nothing for autograd: the gradient is the caller's to ask for. ``out`` may be
+    x; otherwise the two must not overlap."""
     entry = "th_rope"
     shape = n, width = _heads(x, head_dim, entry, "x")
     dev, dt, pt, half = x.get_device(), x.dtype, positions.dtype, freqs.numel()

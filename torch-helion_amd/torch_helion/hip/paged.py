@@ -146,9 +146,11 @@ class PagedKVCache:
     int32 page table [rows, ceil(max_len / page_size)] on the device, -1 past each row's pages.
 
     ``dtype`` is torch.bfloat16 or torch.float8_e4m3fn; an e4m3 cache may have scales, fp32
-    [layers, kv_heads]. ``page_size`` is a power of two of at least 16. Calls work on the current
-    stream; ``extend``, ``fork`` and ``compact`` change the table there, so calls that read it must
-    be ordered with them, as calls on one stream are."""
+    [layers, kv_heads]. ``page_size`` is a power of two of at least 16; ``attend`` takes a
+    ``head_dim`` of 64 or 128, the other calls any up to 1024. Calls work on the current stream;
+    ``extend``, ``fork``, ``shrink``, ``close`` and ``compact`` change the table there, so calls that
+    read it must be ordered with them, as calls on one stream are. An ``extend`` that needs pages and
+    a ``compact`` that moves some copy their page numbers from the host and wait for the stream."""
 
     def __init__(self, *, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int, rows: int, max_len: int,
                  dtype: torch.dtype = torch.bfloat16, device: int | torch.device = 0, k_scale: torch.Tensor | None = None,
