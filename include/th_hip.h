@@ -370,7 +370,7 @@ int th_paged_append(const th_paged_append_desc* desc, void* stream);
  * unseen keys hold, NaN included, does not reach the result. The keys of all
  * tokens are dealt out evenly over the GPU, whatever the lengths, and the
  * parts are joined through the workspace (which short rows do not need). Sums
- * and maxima are fp32; a softmax's numerators meet the values off by 2^-16 over a
+ * and maxima are fp32; a softmax's numerators meet the values off by 2^-15 over a
  * bf16 cache, by 2^-11 (or 2^-39 of the largest) over an e4m3 one. o may be q
  * (same row stride).
  */

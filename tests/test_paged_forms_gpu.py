@@ -54,8 +54,9 @@ def attention64(q, kc, vc, table, pos, rows, scale, window=0, softcap=0.0, slope
 
 def p_step(cache) -> float:
     """What a probability of the second product is off by, relative to it: two bf16 halves over a bf16
-    cache (the second one's half step of what the first left over), one fp16 over an e4m3 cache."""
-    return u(BF16) ** 2 if cache == BF16 else u(torch.float16)
+    cache (the second one's half step of what the first left over, at most 2^-7: it is taken 2^-8 below p
+    and rounded), one fp16 over an e4m3 cache."""
+    return u(BF16) * 2.0 ** -7 if cache == BF16 else u(torch.float16)
 
 
 # ------------------------------------------------------------------ probabilities
@@ -106,6 +107,27 @@ def test_many_keys_of_little_weight_are_not_lost(gpu, cache, top, room):
         tol = tol + room * 2.0 ** -39 * 448.0
     assert (tol < 0.05 * ref).all()
     assert_within(out.view(1, 1, d), ref, tol)
+
+
+@pytest.mark.parametrize("room", [64, 8192])
+@pytest.mark.parametrize("n,amplitude", [(1, 1.0), (2, 0.0), (60, 0.0), (60, 1.0), (33, 4.0)])
+def test_infinite_values_stay_infinite(gpu, n, amplitude, room):
+    """An infinity among the values a token sees is its output there, of its sign; the other dims are finite. Weights
+    of one key alone, of equal keys (powers of two, whose second half is none) and of any."""
+    from torch_helion.hip import ops
+
+    announce(f"paged attention, infinite values, {n} keys room={room} amplitude={amplitude}")
+    d = 64
+    kc, vc, table = paged(1, room // 16, 16, 2, d, BF16, gen(n), gpu)
+    page = int(table[0, (n - 1) // 16])
+    vc[page, (n - 1) % 16, :, 3], vc[page, (n - 1) % 16, :, 40] = float("inf"), float("-inf")
+    q = (torch.randn(1, 8 * d, generator=gen(5)) * amplitude).to(BF16).to(gpu)
+    out = torch.empty_like(q)
+    ops.paged_attention(q, kc, vc, table, torch.tensor([n - 1], dtype=torch.int32, device=gpu), out, scale=d ** -0.5)
+    out = out.view(8, d).float().cpu()
+    assert (out[:, 3] == float("inf")).all() and (out[:, 40] == float("-inf")).all()
+    out[:, 3] = out[:, 40] = 0.0
+    assert torch.isfinite(out).all()
 
 
 @pytest.mark.parametrize("room", [64, 8192])

@@ -36,13 +36,14 @@
 //            ones serve two k steps, q alike): 100.3 us, through the slice 101.6.
 //   O^T      += V^T P^T: V is read transposed (ds_read_b64_tr_b16); P^T is the S^T
 //            accumulators as they are, sums and maxima stay fp32. With a bf16 V each
-//            p goes in as two bf16 halves, h + (p - h): off by 2^-16 of it. One half
-//            (2^-8) took the error against 64 bits from 0.0017, the output's own
-//            rounding, to 0.0020-0.0022, for 133.2 us instead of 133.8 (64 sequences
-//            of 2048-4096 keys), 17.1 instead of 17.7 (23 windows of 1000, 12 heads of
-//            64). An e4m3 V is staged as fp16, which holds it exactly, and p is one
-//            fp16 (2^-11: error 0.0017): 95.9 us, as with one bf16 half (0.0021); two
-//            halves 100.3.
+//            p goes in as two bf16 halves, h + (p - h): off by 2^-15 of it. h is less
+//            than p, so that p - h is above zero and an infinite value stays one (0 inf
+//            and inf - inf are NaN). One half (2^-8) took the error against 64 bits
+//            from 0.0017, the output's own rounding, to 0.0020-0.0022, for 132.5 us
+//            instead of 133.3 (64 sequences of 2048-4096 keys), 17.2 instead of 18.0
+//            (23 windows of 1000, 12 heads of 64). An e4m3 V is staged as fp16, which
+//            holds it exactly, and p is one fp16 (2^-11: error 0.0017): 95.9 us, as with
+//            one bf16 half (0.0021); two halves 100.3.
 // The next tile's loads are issued as soon as this one has left its registers, and
 // land during the softmax and the second product. Buffer loads return zero past
 // their range: unseen slots of a page and pages outside the cache cost no branch, and
@@ -547,7 +548,7 @@ __global__ void __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2,
           if constexpr (E4) {
             pf[b / 2][i] = (_Float16)e;
           } else {
-            const __bf16 h = (__bf16)e;
+            const __bf16 h = (__bf16)(e * 0.99609375f);  // 1 - 2^-8: less than e when rounded
             pf[b / 2][i] = h;
             pl[b / 2][i] = (__bf16)(e - (float)h);
           }
