@@ -6,17 +6,19 @@
 // bytes, so nothing is converted on the way. Weights are the first operand: a
 // lane then holds four consecutive columns n of one row m.
 //
-// Of e2m1 activations the products and the sums of 16 of them are exact in the matrix cores, of e4m3 ones what lies more
-// than 13 bits below the largest product of 16 consecutive k is cut off (measured with single values); the sums are fp32.
-// That is some 2e-6 of a sum: nothing next to a bf16 result's rounding, and of the SwiGLU's e4m3 codes about one in 18000
-// falls on the other side of a rounding. The plain formula's alternative, products in bf16, has a quarter of the rate.
-// (The 32x32x64 form has the same rate on zeros, and 3.98 against 4.73 PFLOP/s on random values: power.)
+// The matrix cores add the products of 16 consecutive k at the largest sum E of their operands' exponents (of subnormal
+// values the least exponent; found with pairs of products, all of 8 million as this says) and cut what lies below
+// 2^(E - 13). Of e2m1 activations nothing does. Of e4m3 ones E <= 8 + 2 and bits reach down to 2^-10, so that the values of 2
+// and more and those below are multiplied apart, two products for one: of the former E <= 10 and the last bit is 2^-3, of
+// the latter E <= 2 and 2^-10, and nothing is cut. The sums are fp32. (With one product 16384 x 4096 x 14336 took 690 us
+// for 1115, 64 rows 15.2 for 15.9, and of the SwiGLU's e4m3 codes one in 18000 fell on the other side of a rounding. bf16
+// products have a quarter of the rate, and both operands to convert.)
+// (The 32x32x64 form has the same rate on zeros, and 3.98 against 4.73 PFLOP/s on random values.)
 //
-// What bounds it: with few rows the weights (64 x 4096 x 14336: 31 MB, 6 us at the 5.2 TB/s of a copy; 15.4 us, since each
+// What bounds it: with few rows the weights (64 x 4096 x 14336: 31 MB, 6 us at the 5.2 TB/s of a copy; 15.9 us, since each
 // CU takes in 40 to 50 GB/s of activations and weights), with many the matrix cores and what feeds them:
-// 16384 x 4096 x 14336 690 us (2.79 PFLOP/s), 6001 x 14336 x 4096 of e2m1 235 us (3.0), SwiGLU of 8192 x 14336 x 4096
-// 750 us (2.57), where a library's product of e4m3 matrices of 8192 cubed reaches 2.65 PFLOP/s. Of the first the matrix
-// cores are busy for 73 % of the cycles, at 1.75 GHz: it draws what the card may draw.
+// 16384 x 4096 x 14336 1115 us (1.73 PFLOP/s, of two products each 3.45), SwiGLU of 8192 x 14336 x 4096 1115 (1.73); 6001 x
+// 14336 x 4096 of e2m1 235 us (3.0). Of the first the matrix cores are busy for 79 % of the cycles, at 2.15 GHz.
 //
 // Operand layout of v_mfma_scale_f32_16x16x128_f8f6f4: lane l supplies row l % 16;
 // of e2m1 the 32 values (16 bytes) of k block g = l / 16; of e4m3 the 16 bytes from
@@ -49,6 +51,18 @@ __device__ __forceinline__ mx_v8i mx_wide(uint4 x) { return mx_v8i{(int)x.x, (in
 __device__ __forceinline__ mx_v8i mx_wide(mx_v8i x) { return x; }
 __device__ __forceinline__ mx_v8i mx_wide(uint4 x, uint4 y) {
   return mx_v8i{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
+}
+
+// e4m3 values of 2 and more (exponent fields from 8 on, NaN among them) and those below, in each half zeros of their sign
+// in the others' places.
+__device__ __forceinline__ void mx_split(mx_v8i x, mx_v8i& large, mx_v8i& small) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t v = (uint32_t)x[i], f = v & 0x40404040u;
+    const uint32_t s = v & ~(f | (f - (f >> 6)));  // (0x40 and 0x3f of a large byte)
+    large[i] = (int)(v ^ (s & 0x7f7f7f7fu));
+    small[i] = (int)s;
+  }
 }
 
 // The sums of WAVES waves, [WAVES][ROWS][LDR] in LDS (with SWIGLU the gate's OUTS columns, then the up
@@ -129,21 +143,30 @@ static bool mx_whole_stages(const MxGemmK& k) {
   return k.nb % 4 == 0 && (((uintptr_t)k.as | (uintptr_t)k.ws | (uint64_t)k.ldas | (uint64_t)k.ldws) & 3) == 0;
 }
 
-// Which form takes least time: what a workgroup loads over what a CU takes in (bytes a microsecond, fitted to the
-// times below), in as many rounds as the workgroups need. us by form, e4m3 activations:
-//                           ring   64x64  64x128  128x256  256x256
-//     1 x 6144 x 4096        4.9
-//    64 x 4096 x 4096        6.8
-//   128 x 4096 x 4096       11.0    13.9    16.0     31.0     43.6
-//    64 x 14336 x 4096      21.5    14.6    16.6     29.3     43.5
-//   256 x 4096 x 4096       19.9    14.3    16.4     31.0     46.6
-//   512 x 4096 x 4096       38.0    22.1    17.6     31.3     47.0
-//  2048 x 4096 x 4096      143.4    71.9    53.4     41.0     49.0
-//  2048 x 14336 x 4096     543     267     210      167      128
-//   333 x 2050 x 1376       10.7     7.3     9.7   (43 blocks)
-//  2048 x 4096 x 4064              101      80       50   (127 blocks)
-//  8192 x 4096 x 14304            1335    1016      664   (447 blocks)
-// The choice was within 8 % of the best of 34 such calls.
+// Which form takes least time: what a workgroup loads over what a CU takes in (bytes a microsecond), in as many rounds as
+// the workgroups need. us by form, in a graph:
+//                             e4m3 activations                         e2m1
+//                           ring   64x64  64x128  128x256  256x256     ring   64x64  64x128  128x256  256x256
+//     1 x 6144 x 4096        5.9    15.2    19.7     40.8     71.8
+//    64 x 4096 x 4096        7.1    15.4    20.5     43.2     75.7      5.5    11.3    13.2     21.8     32.1
+//   128 x 4096 x 4096       12.3    15.7    20.7     44.9     76.4      9.2    11.5    14.3     26.7     34.4
+//    64 x 14336 x 4096      23.4    16.6    21.0     43.8     76.5     18.6    12.4    15.3     24.3     34.1
+//   256 x 4096 x 4096       23.3    16.6    21.0     45.0     78.9     17.2    12.2    14.7     26.9     38.5
+//   512 x 4096 x 4096       43.2    22.8    22.1     45.3     79.7     32.2    19.6    16.0     26.9     38.4
+//  1024 x 4096 x 14336     226     129     100      134      238      185     108      79.6     76.1    101
+//  2048 x 4096 x 4096      156      79.4    61.5     52.2     80.9    119      64.5    48.4     32.7     40.1
+//  2048 x 14336 x 4096     584     282     226      214      189      468     239     192      141      110
+//   333 x 2050 x 1376       11.8     8.8    12.3     23.9   (43 blocks)
+//  2048 x 4096 x 4064      180     103      81.6     59.1   (127)     133      85.4    72.7     44.4
+//  8192 x 4096 x 14304            1347    1070      733     (447)
+//  SwiGLU (weights 2 x)
+//     1 x 14336 x 4096      15.9            20.0     40.4     71.6
+//    64 x 14336 x 4096      34.0            20.5     41.4     72.2     30.9            15.7     23.0     30.1
+//   256 x 14336 x 4096     113              57.0     45.0     73.8    103              44.3     27.9     34.8
+//  1024 x 14336 x 4096     444             198      183      157      405             158      108       80.2
+//  8192 x 14336 x 4064                    2058     1484     (127)
+// Of 55 such calls the choice was the best or within 6 % of it in 50, within 14 % in the others (1000 x 4096 x 4096: 37.4, in
+// tiles of 64 x 128 32.8).
 static int mx_form(const MxGemmK& k, bool a4, bool swiglu) {
   const double cus = device_cus() > 0 ? device_cus() : 256, nk = (double)cdiv(k.nb, 4);
   const bool odd = !mx_whole_stages(k);
@@ -237,12 +260,25 @@ struct MxTile {
   static constexpr int SETS = ODD ? 0 : (STAGES + 4) / 2, SET = 8 * (BM + BN), SCALES = STAGES * STAGE;
   static constexpr int LDS = SCALES + SETS * SET;
   static constexpr int PA = ABYTES / 1024, PW = WBYTES / 1024, SP = (BM + BN) / (ODD ? 16 : 64);  // loads: 1 KiB, 32 rows of scales (ODD: 16)
+  static constexpr int GROUP = TN > 8 ? TN / 4 : TN / 2;  // column subtiles multiplied while the next are read
   static constexpr int share(int n) { return (n + WAVES - 1) / WAVES; }  // of them a wave issues
   static constexpr int LA = share(PA), LW = share(PW), LS = share(SP), LOADS = LA + LW + LS;
   static_assert(BM % 64 == 0 && OUTS % 64 == 0 && TN % 4 == 0, "tile shape");
   static_assert(STAGES >= 3 && (STAGES - 1) * LOADS < 64, "stages, vmcnt");
   static_assert(LDS <= 160 * 1024, "LDS");
 };
+
+// The order of what stands between two points that nothing moves across: N times a product, then READS reads of LDS and
+// VALU vector instructions.
+template <int N, int READS, int VALU>
+__device__ __forceinline__ void mx_interleave() {
+  if constexpr (N > 0) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    if constexpr (READS > 0) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    if constexpr (VALU > 0) __builtin_amdgcn_sched_group_barrier(0x002, VALU, 0);
+    mx_interleave<N - 1, READS, VALU>();
+  }
+}
 
 template <bool A4, bool SWIGLU, bool ODD, int TM, int TN, int WM, int WN, int STAGES>
 __global__ void __launch_bounds__(64 * WM * WN) mx_gemm_tile_kernel(MxGemmK p, int tiles_m, int tiles_n) {
@@ -375,7 +411,8 @@ __global__ void __launch_bounds__(64 * WM * WN) mx_gemm_tile_kernel(MxGemmK p, i
   f32x4_t acc[TN][TM] = {};
   uint4 fw[TN];
   std::conditional_t<A4, uint4, mx_v8i> fa[TM];
-  int cw[TN], ca[TM];  // scales
+  mx_v8i large[TM], small[TM];  // of e4m3
+  int cw[TN], ca[TM], cn[TM];  // scales; of fa
   auto scale_of = [&](int row, int kt, int st) {
     if constexpr (ODD) return (int)*(const uint8_t*)(smem + st * T::STAGE + T::ABYTES + T::WBYTES + row * 16 + 4 * g);
     else return (int)*(const uint8_t*)(smem + T::SCALES + (kt >> 1) % T::SETS * T::SET + 4 * (kt & 1) + row * 8 + g);
@@ -384,34 +421,62 @@ __global__ void __launch_bounds__(64 * WM * WN) mx_gemm_tile_kernel(MxGemmK p, i
     const char* b = smem + st * T::STAGE + (wm * TM + j) * 16 * (A4 ? 64 : 128);
     if constexpr (A4) fa[j] = *(const uint4*)(b + oa[0]);
     else fa[j] = mx_wide(*(const uint4*)(b + oa[0]), *(const uint4*)(b + oa[1]));
-    ca[j] = scale_of((wm * TM + j) * 16 + r, kt, st);
+    cn[j] = scale_of((wm * TM + j) * 16 + r, kt, st);
+    if constexpr (A4) ca[j] = cn[j];
   };
   auto read_w = [&](int i, int kt, int st) __attribute__((always_inline)) {
     fw[i] = *(const uint4*)(smem + st * T::STAGE + T::ABYTES + (wfirst(i) - 4 * (i & 1)) * 64 + ow[i & 1]);
     cw[i] = scale_of(T::BM + wfirst(i) + rw, kt, st);
   };
-  auto multiply = [&](int i0, int j) __attribute__((always_inline)) {
+  auto product = [&](int i0, int j, mx_v8i a) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = i0; i < i0 + TN / 2; ++i)
-      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_wide(fw[i]), mx_wide(fa[j]), acc[i][j], 4, A4 ? 4 : 0, 0,
-                                                                   cw[i], 0, ca[j]);
+    for (int i = i0; i < i0 + T::GROUP; ++i)
+      acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_wide(fw[i]), a, acc[i][j], 4, A4 ? 4 : 0, 0, cw[i], 0, ca[j]);
+  };
+  auto multiply = [&](int i0, int j) __attribute__((always_inline)) {
+    if constexpr (A4) {
+      product(i0, j, mx_wide(fa[j]));
+    } else {
+      product(i0, j, small[j]);
+      product(i0, j, large[j]);
+    }
+  };
+  auto split = [&](int j) __attribute__((always_inline)) {
+    if constexpr (!A4) mx_split(fa[j], large[j], small[j]);
+    ca[j] = cn[j];
   };
   // (Touching lines ahead into L2, starting the workgroups at different stages, and four waves of 128 x 128 gained
-  // nothing: the loads alone take 1.47 us a stage of 256 x 256, the products alone 0.92, both together 1.5.)
-  // A stage: the first half of its weights is multiplied while the second half is read. Then every wave has the stage
-  // in registers, and while the second half is multiplied its place is refilled, the next stage's first half is
-  // read, and its activations as they are done with. All of that goes between the products: the two waves of a SIMD
-  // meet at the barrier, and what stands before their next products leaves the matrix cores idle.
-  constexpr int H = TN / 2;
+  // nothing.)
+  // A stage: a group of its weights' subtiles is multiplied while the next is read. Once the last group is read every wave
+  // has the stage in registers, and while that group is multiplied the stage's place is refilled, the next stage's first
+  // group is read, and its activations. All of that goes between the products: the two waves of a SIMD meet at the
+  // barrier, and what stands before their next products leaves the matrix cores idle. e4m3 activations are split there too,
+  // once a stage for all columns: so a wave has few row subtiles and many column subtiles (256 x 256: 2 and 16, 1115 us; 4 and
+  // 8, split for every group, 1196).
+  constexpr int H = T::GROUP;
   int st = 0;
   auto stage = [&](int kt) __attribute__((always_inline)) {
+    if constexpr (A4) {
 #pragma unroll
-    for (int j = 0; j < TM; ++j) {
-      multiply(0, j);
-      __builtin_amdgcn_sched_barrier(0);
+      for (int j = 0; j < TM; ++j) {
+        multiply(0, j);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = j * H / TM; i < (j + 1) * H / TM; ++i) read_w(H + i, kt, st);
-      __builtin_amdgcn_sched_barrier(0);
+        for (int i = j * H / TM; i < (j + 1) * H / TM; ++i) read_w(H + i, kt, st);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+#pragma unroll
+      for (int p = 0; p < TN - H; p += H) {
+#pragma unroll
+        for (int i = 0; i < H; ++i) read_w(p + H + i, kt, st);
+        if (p == 0) split(TM - 1);
+#pragma unroll
+        for (int j = 0; j < TM; ++j) multiply(p, j);
+        if (p == 0) mx_interleave<2 * H, 1, (TM > 1 ? 40 / (2 * H) : 0)>();
+        else mx_interleave<2 * H, 1, 0>();
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
     // the next stage's loads of this wave have landed, those of later ones stay in flight; after the barrier
     // every wave's have
@@ -420,15 +485,31 @@ __global__ void __launch_bounds__(64 * WM * WN) mx_gemm_tile_kernel(MxGemmK p, i
     const int now = st;
     st = st == STAGES - 1 ? 0 : st + 1;
     mend(kt + 1, st);
+    // (behind the last stage what is read is not used)
 #pragma unroll
     for (int j = 0; j < TM; ++j) {
-      multiply(H, j);
-      __builtin_amdgcn_sched_barrier(0);
-      // (behind the last stage what is read is not used)
+      if constexpr (!A4) {
+        if (j == 0) {
 #pragma unroll
-      for (int i = j * H / TM; i < (j + 1) * H / TM; ++i) read_w(i, kt + 1, st);
-      read_a(j, kt + 1, st);
+          for (int i = 0; i < TM; ++i) read_a(i, kt + 1, st);
+#pragma unroll
+          for (int i = 0; i < H; ++i) read_w(i, kt + 1, st);
+        } else {
+          split(j - 1);
+        }
+      }
+      multiply(TN - H, j);
+      if constexpr (!A4) {
+        if (j == 0) mx_interleave<2 * H, (3 * TM + 2 * H + 2 * H - 1) / (2 * H), 0>();
+        else mx_interleave<2 * H, 0, 40 / (2 * H)>();
+      }
       __builtin_amdgcn_sched_barrier(0);
+      if constexpr (A4) {
+#pragma unroll
+        for (int i = j * H / TM; i < (j + 1) * H / TM; ++i) read_w(i, kt + 1, st);
+        read_a(j, kt + 1, st);
+        __builtin_amdgcn_sched_barrier(0);
+      }
       // (near the end the last stage again, which nobody reads: the number in flight stays the same)
 #pragma unroll
       for (int i = j * T::LOADS / TM; i < (j + 1) * T::LOADS / TM; ++i) load(i, min(kt + STAGES, nk - 1), now);
@@ -452,7 +533,10 @@ __global__ void __launch_bounds__(64 * WM * WN) mx_gemm_tile_kernel(MxGemmK p, i
 #pragma unroll
   for (int i = 0; i < H; ++i) read_w(i, 0, 0);
 #pragma unroll
-  for (int j = 0; j < TM; ++j) read_a(j, 0, 0);
+  for (int j = 0; j < TM; ++j) {
+    read_a(j, 0, 0);
+    if (j < TM - 1) split(j);
+  }
 #pragma unroll 1
   for (int kt = 0; kt < nk; ++kt) stage(kt);
   wait_vmcnt<0>();
@@ -496,14 +580,15 @@ __global__ void __launch_bounds__(64 * WM * WN) mx_gemm_tile_kernel(MxGemmK p, i
       }
     }
   } else {
-    // the residual of a row subtile is loaded ahead of the stores of the one before: one round trip, not one a store
-    // (it may be out itself, so the compiler keeps the order as it is written)
-    float to[NP][8];
-    auto load_residual = [&](int j) __attribute__((always_inline)) {
-      const int mrow = (wm * TM + j) * 16 + r;
+    // the residual of four pairs of a row subtile is loaded ahead of the stores of the four before: one round trip, not one a
+    // store (it may be out itself, so the compiler keeps the order as it is written)
+    constexpr int NR = NP < 4 ? NP : 4, PARTS = NP / NR;
+    float to[NR][8];
+    auto load_residual = [&](int part) __attribute__((always_inline)) {
+      const int mrow = (wm * TM + part / PARTS) * 16 + r;
 #pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        const int c = column(i);
+      for (int i = 0; i < NR; ++i) {
+        const int c = column(part % PARTS * NR + i);
 #pragma unroll
         for (int e = 0; e < 8; ++e) to[i][e] = 0.f;
         if (!p.res || mrow >= mrows || c >= nouts) continue;
@@ -533,16 +618,17 @@ __global__ void __launch_bounds__(64 * WM * WN) mx_gemm_tile_kernel(MxGemmK p, i
     };
     load_residual(0);
 #pragma unroll
-    for (int j = 0; j < TM; ++j) {
+    for (int part = 0; part < TM * PARTS; ++part) {
+      const int j = part / PARTS, i0 = part % PARTS * NR;
 #pragma unroll
-      for (int i = 0; i < NP; ++i)
+      for (int i = 0; i < NR; ++i)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) acc[2 * i + (e >> 2)][j][e & 3] += to[i][e];
-      if (j + 1 < TM) load_residual(j + 1);
+        for (int e = 0; e < 8; ++e) acc[2 * (i0 + i) + (e >> 2)][j][e & 3] += to[i][e];
+      if (part + 1 < TM * PARTS) load_residual(part + 1);
       const int mrow = (wm * TM + j) * 16 + r;
       if (mrow >= mrows) continue;
 #pragma unroll
-      for (int i = 0; i < NP; ++i) {
+      for (int i = i0; i < i0 + NR; ++i) {
         const int c = column(i);
         if (c >= nouts) continue;
         const int64_t at = (m0 + mrow) * p.ldo + n0 + c;
@@ -713,14 +799,25 @@ __global__ void __launch_bounds__(512) mx_gemm_ring_kernel(MxGemmK p) {
     wait_lgkmcnt0();  // the stage is in registers: its place may be filled again
     mx_lds_order();
     if (it + STAGES < mine) issue(wave + WAVES * (it + STAGES), st);
+    auto product = [&](auto half, mx_v8i x) __attribute__((always_inline)) {
+      constexpr int s = decltype(half)::value;
 #pragma unroll
-    for (int t = 0; t < TN; ++t)
-      acc[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_wide(w[t][0]), A4 ? mx_wide(a[0][0]) : mx_wide(a[0][0], a[0][A4 ? 0 : 1]),
-                                                               acc[t], 4, A4 ? 4 : 0, 0, sw[t], 0, sa);
-#pragma unroll
-    for (int t = 0; t < TN; ++t)
-      acc[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_wide(w[t][1]), A4 ? mx_wide(a[1][0]) : mx_wide(a[1][0], a[1][A4 ? 0 : 1]),
-                                                               acc[t], 4, A4 ? 4 : 0, 1, sw[t], 1, sa);
+      for (int t = 0; t < TN; ++t)
+        acc[t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_wide(w[t][s]), x, acc[t], 4, A4 ? 4 : 0, s, sw[t], s, sa);
+    };
+    auto multiply = [&](auto half) __attribute__((always_inline)) {
+      constexpr int s = decltype(half)::value;
+      if constexpr (A4) {
+        product(half, mx_wide(a[s][0]));
+      } else {
+        mx_v8i large, small;
+        mx_split(mx_wide(a[s][0], a[s][1]), large, small);
+        product(half, small);
+        product(half, large);
+      }
+    };
+    multiply(std::integral_constant<int, 0>());
+    multiply(std::integral_constant<int, 1>());
     st = st == STAGES - 1 ? 0 : st + 1;
   }
   __syncthreads();  // the rings are done with
@@ -767,13 +864,13 @@ static void launch_gemm(const MxGemmK& k, int form, hipStream_t s) {
       else launch_tile<A4, false, false, 1, 4, 4, 1, 4>(k, s);
     }
   } else if (form == kMxTile64w) {
-    if (odd) launch_tile<A4, SWIGLU, true, 2, 4, 2, 2, 4>(k, s);
-    else launch_tile<A4, SWIGLU, false, 2, 4, 2, 2, 4>(k, s);
+    if (odd) launch_tile<A4, SWIGLU, true, A4 ? 2 : 1, A4 ? 4 : 8, A4 ? 2 : 4, A4 ? 2 : 1, 4>(k, s);
+    else launch_tile<A4, SWIGLU, false, A4 ? 2 : 1, A4 ? 4 : 8, A4 ? 2 : 4, A4 ? 2 : 1, 4>(k, s);
   } else if (form == kMxTile128) {
-    if (odd) launch_tile<A4, SWIGLU, true, 4, 4, 2, 4, 4>(k, s);
-    else launch_tile<A4, SWIGLU, false, 4, 4, 2, 4, 4>(k, s);
+    if (odd) launch_tile<A4, SWIGLU, true, A4 ? 4 : 2, A4 ? 4 : 8, A4 ? 2 : 4, A4 ? 4 : 2, 4>(k, s);
+    else launch_tile<A4, SWIGLU, false, A4 ? 4 : 2, A4 ? 4 : 8, A4 ? 2 : 4, A4 ? 4 : 2, 4>(k, s);
   } else {
-    launch_tile<A4, SWIGLU, false, 4, 8, 4, 2, A4 ? 4 : 3>(k, s);
+    launch_tile<A4, SWIGLU, false, A4 ? 4 : 2, A4 ? 8 : 16, A4 ? 4 : 8, A4 ? 2 : 1, A4 ? 4 : 3>(k, s);
   }
 }
 
