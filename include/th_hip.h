@@ -519,6 +519,21 @@ typedef struct th_mx_gemm_desc {
 
 int th_mx_gemm(const th_mx_gemm_desc* desc, void* stream);
 
+/* The form in which th_mx_gemm runs this descriptor, by its sizes and the
+ * alignment of its scales: form[0] a th_mx_form, form[1] 1 where scales are loaded
+ * byte by byte (blocks is no multiple of four, or scale rows do not start at
+ * whole dwords). Launches nothing and reads no operand; without an initialised
+ * device, for 256 compute units. */
+typedef enum th_mx_form {
+  TH_MX_RING = 0,          /* 32 columns a workgroup, k dealt out to its waves */
+  TH_MX_TILE_64X64 = 1,    /* tiles of rows x rows of w */
+  TH_MX_TILE_64X128 = 2,
+  TH_MX_TILE_128X256 = 3,
+  TH_MX_TILE_256X256 = 4
+} th_mx_form;
+
+int th_mx_gemm_form(const th_mx_gemm_desc* desc, int32_t* form);
+
 /* ------------------------------------------------------------ SSD scan
  * The Mamba-2 scan, per (batch b, head h) over token-major operands:
  *   y_t = sum_{s<=t} (C_t . B_s) exp(cum_t - cum_s) dt_s x_s + D_h x_t  [* gate_t]

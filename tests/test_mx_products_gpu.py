@@ -14,6 +14,7 @@ import torch
 
 import mx_oracle
 from conftest import announce
+from test_mx_forms_gpu import FORMS, size_of
 
 pytestmark = pytest.mark.gpu
 
@@ -35,13 +36,10 @@ def unit(rows, k, gpu, s=127):
     return torch.full((rows, k // 32), s, dtype=torch.uint8, device=gpu)
 
 
-# (one to 32 rows; a few hundred; thousands; widths of whole stages of 128 values and others)
-SIZES = [(1, 70, 128), (8, 64, 640), (9, 64, 672), (16, 100, 640), (40, 300, 640), (33, 64, 608), (256, 4096, 640), (333, 2050, 672),
-         (512, 4096, 640), (600, 4100, 608), (1900, 4200, 384), (1000, 4200, 672), (2000, 4100, 608), (3000, 5200, 640)]
-
-
-@pytest.mark.parametrize("m,n,k", SIZES)
-def test_small_products_beside_large_ones_keep_their_bits(gpu, m, n, k):
+# (widths of whole stages of four blocks, and of others)
+@pytest.mark.parametrize("form,nb", [*((f, 19) for f in FORMS if f != "256x256"), *((f, 20) for f in FORMS), ("64x128", 4)])
+def test_small_products_beside_large_ones_keep_their_bits(gpu, form, nb):
+    (m, n), k = size_of(form, nb, 8, False, False), 32 * nb
     from torch_helion.hip import ops
 
     announce(f"mx_gemm exact sums m={m} n={n} k={k}")
@@ -54,13 +52,13 @@ def test_small_products_beside_large_ones_keep_their_bits(gpu, m, n, k):
     assert off == 0.0, f"off by {off:.3e}"
 
 
-@pytest.mark.parametrize("m,f,k", [(3, 64, 640), (16, 96, 640), (40, 160, 608), (64, 14336, 640), (200, 4096, 608), (1000, 4096, 672),
-                                   (1000, 4096, 640), (2048, 4096, 640)])
-def test_swiglu_of_exact_sums(gpu, m, f, k):
+@pytest.mark.parametrize("form,nb", [(f, nb) for f in FORMS for nb in (19, 20) if f != "64x64" and (f, nb) != ("256x256", 19)])
+def test_swiglu_of_exact_sums(gpu, form, nb):
     """The sums in units of 2^-12: gates of a few units, whose SwiGLU is off by (|g| + 8) 2^-23 of itself at most (the exponential's
     argument is rounded once: |g| 2^-24, and two more steps; then the sum, the reciprocal and two products)."""
     from torch_helion.hip import ops
 
+    (m, f), k = size_of(form, nb, 8, True, False), 32 * nb
     announce(f"mx_swiglu of exact sums m={m} f={f} k={k}")
     ac, a, wc, w = operands(m, 2 * f, k, m + f + k)
     a, w = a.to(gpu), w.to(gpu)
@@ -72,17 +70,17 @@ def test_swiglu_of_exact_sums(gpu, m, f, k):
     mx_oracle.assert_blocks_within(codes, scales, y, (g.abs() + 8) * 2.0 ** -23 * y.abs(), 8)
 
 
-@pytest.mark.parametrize("m,n", [(1, 70), (16, 96), (300, 300), (3000, 5200)])
-def test_every_value_beside_every_other(gpu, m, n):
+@pytest.mark.parametrize("form,k", [*((f, 128) for f in FORMS if f != "256x256"), ("256x256", 640)])
+def test_every_value_beside_every_other(gpu, form, k):
     """Blocks of any finite codes: off for each of two products of matrices by the 2^-22 of the magnitudes that a scaled
     MFMA's result is taken to be off by."""
     from torch_helion.hip import ops
 
-    k = 128
+    m, n = size_of(form, k // 32, 8, False, False)
     announce(f"mx_gemm of any codes m={m} n={n}")
     g = torch.Generator().manual_seed(m)
     a = torch.randint(0, 0x7f, (m, k), generator=g, dtype=torch.uint8) + 0x80 * torch.randint(0, 2, (m, k), generator=g, dtype=torch.uint8)
-    a[:, 32:] = 0    # (one block: a stage of its own, of which the others are zeros)
+    a[:, 32:] = 0    # (one block: the other products are zeros)
     a = a.view(E4M3)
     wc = torch.randint(0, 256, (n, k // 2), generator=g, dtype=torch.uint8)
     x, w = a.double().to(gpu), mx_oracle.elements(wc).flatten(1).to(gpu)

@@ -135,9 +135,6 @@ __device__ __forceinline__ void mx_finish(const MxGemmK& p, const float* red, in
   }
 }
 
-// Forms: the ring of few rows, and tiles of 64 x 64, 64 x 128, 128 x 256 and 256 x 256.
-enum { kMxRing, kMxTile64, kMxTile64w, kMxTile128, kMxTile256 };
-
 // Rows of whole stages of four blocks, their scales whole dwords. (Else the scales are loaded byte by byte.)
 static bool mx_whole_stages(const MxGemmK& k) {
   return k.nb % 4 == 0 && (((uintptr_t)k.as | (uintptr_t)k.ws | (uint64_t)k.ldas | (uint64_t)k.ldws) & 3) == 0;
@@ -173,22 +170,22 @@ static int mx_form(const MxGemmK& k, bool a4, bool swiglu) {
   const double ka = a4 ? 64 : 128;
   auto rounds = [&](double groups, double at_once) { return (double)cdiv((int64_t)groups, (int64_t)at_once); };
   double best = 1e30;
-  int form = kMxTile256;
+  int form = TH_MX_TILE_256X256;
   auto offer = [&](int f, double us) {
     if (us < best) best = us, form = f;
   };
   const int sides = swiglu ? 2 : 1;
   const double rows = (double)std::min<int64_t>(k.M, k.M <= 8 ? 8 : k.M <= 16 ? 16 : 32);
-  if (k.M <= 4096) offer(kMxRing, 3.0 + rounds(cdiv(k.N, 32) * cdiv(k.M, 32), cus) * nk * (rows * ka + 2200.0 * sides) / (odd ? 35e3 : 50e3));
+  if (k.M <= 4096) offer(TH_MX_RING, 3.0 + rounds(cdiv(k.N, 32) * cdiv(k.M, 32), cus) * nk * (rows * ka + 2200.0 * sides) / (odd ? 35e3 : 50e3));
   auto tile = [&](int f, int bm, int bn, double per_cu, double rate, double fixed) {
     const double n = (double)(cdiv(k.M, bm) * cdiv(k.N, bn / sides)), load = nk * (bm * ka + bn * 64.0 + 4.0 * (bm + bn));
     offer(f, fixed + (n <= cus ? load / rate : rounds(n, per_cu * cus) * per_cu * load / rate));
   };
-  if (!swiglu) tile(kMxTile64, 64, 64, 2, odd ? 33e3 : 40e3, 3);
-  tile(kMxTile64w, 64, 128, 2, odd ? 29e3 : 40e3, 3);
-  tile(kMxTile128, 128, 256, 1, odd ? 25e3 : 34e3, 4);
+  if (!swiglu) tile(TH_MX_TILE_64X64, 64, 64, 2, odd ? 33e3 : 40e3, 3);
+  tile(TH_MX_TILE_64X128, 64, 128, 2, odd ? 29e3 : 40e3, 3);
+  tile(TH_MX_TILE_128X256, 128, 256, 1, odd ? 25e3 : 34e3, 4);
   if (odd) return form;
-  tile(kMxTile256, 256, 256, 1, 33e3, 6);
+  tile(TH_MX_TILE_256X256, 256, 256, 1, 33e3, 6);
   return form;
 }
 
@@ -855,18 +852,18 @@ static void launch_ring(const MxGemmK& k, hipStream_t s) {
 template <bool A4, bool SWIGLU>
 static void launch_gemm(const MxGemmK& k, int form, hipStream_t s) {
   const bool odd = !mx_whole_stages(k);
-  if (form == kMxRing) {
+  if (form == TH_MX_RING) {
     if (odd) launch_ring<A4, SWIGLU, true>(k, s);
     else launch_ring<A4, SWIGLU, false>(k, s);
-  } else if (form == kMxTile64) {
+  } else if (form == TH_MX_TILE_64X64) {
     if constexpr (!SWIGLU) {
       if (odd) launch_tile<A4, false, true, 1, 4, 4, 1, 4>(k, s);
       else launch_tile<A4, false, false, 1, 4, 4, 1, 4>(k, s);
     }
-  } else if (form == kMxTile64w) {
+  } else if (form == TH_MX_TILE_64X128) {
     if (odd) launch_tile<A4, SWIGLU, true, A4 ? 2 : 1, A4 ? 4 : 8, A4 ? 2 : 4, A4 ? 2 : 1, 4>(k, s);
     else launch_tile<A4, SWIGLU, false, A4 ? 2 : 1, A4 ? 4 : 8, A4 ? 2 : 4, A4 ? 2 : 1, 4>(k, s);
-  } else if (form == kMxTile128) {
+  } else if (form == TH_MX_TILE_128X256) {
     if (odd) launch_tile<A4, SWIGLU, true, A4 ? 4 : 2, A4 ? 4 : 8, A4 ? 2 : 4, A4 ? 4 : 2, 4>(k, s);
     else launch_tile<A4, SWIGLU, false, A4 ? 4 : 2, A4 ? 4 : 8, A4 ? 2 : 4, A4 ? 4 : 2, 4>(k, s);
   } else {
@@ -878,7 +875,7 @@ static void launch_gemm(const MxGemmK& k, int form, hipStream_t s) {
 
 using namespace th;
 
-extern "C" int th_mx_gemm(const th_mx_gemm_desc* d, void* stream) {
+static int check(const th_mx_gemm_desc* d) {
   TH_CHECK_ARG(d != nullptr, "th_mx_gemm: null descriptor");
   TH_CHECK_ARG(d->rows >= 0 && d->rows <= 1 << 21 && d->outs > 0 && d->outs <= 1 << 24 && d->blocks > 0 && d->blocks <= 1 << 18,
                "th_mx_gemm: rows=%lld (at most 2^21) outs=%d (2^24) blocks=%d (2^18) out of range", (long long)d->rows,
@@ -910,7 +907,32 @@ extern "C" int th_mx_gemm(const th_mx_gemm_desc* d, void* stream) {
     TH_CHECK_ARG(d->residual != d->out || d->ld_residual == d->ld_out || d->rows <= 1,
                  "th_mx_gemm: in place needs one row stride");
   }
-  if (d->rows == 0) return TH_OK;
+  return TH_OK;
+}
+
+static MxGemmK operands(const th_mx_gemm_desc* d) {
+  MxGemmK k{};
+  k.M = d->rows; k.N = d->outs; k.nb = d->blocks;
+  k.a = (const uint8_t*)d->a; k.lda = d->ld_a; k.as = d->a_scales; k.ldas = d->ld_a_scales;
+  k.w = (const uint8_t*)d->w; k.ldw = d->ld_w; k.ws = d->w_scales; k.ldws = d->ld_w_scales;
+  k.res = d->residual; k.ldr = d->ld_residual; k.o = d->out; k.ldo = d->ld_out; k.os = d->out_scales; k.ldos = d->ld_out_scales;
+  k.out32 = d->out_dtype == TH_F32; k.e2m1 = d->out_dtype == TH_F4E2M1;
+  return k;
+}
+
+extern "C" int th_mx_gemm_form(const th_mx_gemm_desc* d, int32_t* form) {
+  const int status = check(d);
+  if (status != TH_OK) return status;
+  TH_CHECK_ARG(form != nullptr, "th_mx_gemm_form: null pointer");
+  const MxGemmK k = operands(d);
+  form[0] = mx_form(k, d->a_dtype == TH_F4E2M1, d->swiglu);
+  form[1] = !mx_whole_stages(k);
+  return TH_OK;
+}
+
+extern "C" int th_mx_gemm(const th_mx_gemm_desc* d, void* stream) {
+  const int status = check(d);
+  if (status != TH_OK || d->rows == 0) return status;
   TH_CHECK_ARG(d->a && d->a_scales && d->w && d->w_scales && d->out && (!d->swiglu || d->out_scales),
                "th_mx_gemm: null tensor pointer");
   TH_CHECK_ARG(d->out != d->a && d->out != d->w && (!d->swiglu || d->out != (const void*)d->out_scales),
@@ -919,12 +941,8 @@ extern "C" int th_mx_gemm(const th_mx_gemm_desc* d, void* stream) {
     set_error("th_mx_gemm: th_init was not called for the current device");
     return TH_ERR_NOT_INIT;
   }
-  MxGemmK k{};
-  k.M = d->rows; k.N = d->outs; k.nb = d->blocks;
-  k.a = (const uint8_t*)d->a; k.lda = d->ld_a; k.as = d->a_scales; k.ldas = d->ld_a_scales;
-  k.w = (const uint8_t*)d->w; k.ldw = d->ld_w; k.ws = d->w_scales; k.ldws = d->ld_w_scales;
-  k.res = d->residual; k.ldr = d->ld_residual; k.o = d->out; k.ldo = d->ld_out; k.os = d->out_scales; k.ldos = d->ld_out_scales;
-  k.out32 = d->out_dtype == TH_F32; k.e2m1 = d->out_dtype == TH_F4E2M1;
+  const MxGemmK k = operands(d);
+  const bool a4 = d->a_dtype == TH_F4E2M1;
   hipStream_t s = (hipStream_t)stream;
   const int form = mx_form(k, a4, d->swiglu);
   if (d->swiglu) {

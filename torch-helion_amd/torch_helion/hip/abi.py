@@ -26,6 +26,9 @@ TH_ERR_NOT_INIT = -4
 # th_dtype
 TH_F32, TH_BF16, TH_F16, TH_F8E4M3, TH_I32, TH_I64, TH_F4E2M1 = range(7)
 
+# th_mx_form
+MX_RING, MX_TILE_64X64, MX_TILE_64X128, MX_TILE_128X256, MX_TILE_256X256 = range(5)
+
 # th_epi_op
 EPI_ACC, EPI_ROPE, EPI_ROPE_PAIR, EPI_SILU, EPI_SWIGLU, EPI_ADD, EPI_SOFTPLUS_ADD, EPI_MUL = range(8)
 
@@ -264,6 +267,7 @@ SIGNATURES: dict[str, tuple] = {
     "th_mx_dequantize": (_i32, [_p, _p]),
     "th_mx_rmsnorm": (_i32, [_p, _p]),
     "th_mx_gemm": (_i32, [_p, _p]),
+    "th_mx_gemm_form": (_i32, [_p, C.POINTER(_i32)]),
     "th_epilogue_vm": (_i32, [C.POINTER(VmDesc), _p]),
     "th_ssd_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32]),
     "th_ssd_gtile_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),

@@ -687,12 +687,8 @@ def mx_rmsnorm(x: torch.Tensor, gain: torch.Tensor, eps: float, codes: torch.Ten
     _launch(entry, d, dev, kernel)
 
 
-def mx_gemm(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor, *,
-            residual: torch.Tensor | None = None, kernel: str | None = None) -> torch.Tensor:
-    """out[m, n] = sum_k a[m, k] w[n, k] (+ residual[m, n]): activations in e4m3 or e2m1 blocks,
-    weights in e2m1 blocks ([outs, k], one row an output column), fp32 sums, out and residual bf16 or
-    fp32 of one type. ``residual`` may be ``out``. k is whole blocks: what :func:`mx_quantize` filled up with zeros adds
-    nothing."""
+def _mx_gemm_desc(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor,
+                  residual: torch.Tensor | None) -> tuple[bytes, int]:
     entry = "th_mx_gemm"
     rows, outs, ot, op, ldo = _matrix(out, entry, "out")
     if len(a_scales.shape) != 2:
@@ -705,17 +701,12 @@ def mx_gemm(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales: 
     rp = ldr = 0
     if residual is not None:
         rp, ldr = _rows_of(residual, rows, outs, out.dtype, dev, entry, "residual")
-    d = _pack(entry, _MXG, rows, outs, blocks, at, ot, 0, 0, ap, lda, asp, ldas, wp, ldw, wsp, ldws, rp, ldr, op, ldo,
-              0, 0)
-    _launch(entry, d, dev, kernel)
-    return out
+    return _pack(entry, _MXG, rows, outs, blocks, at, ot, 0, 0, ap, lda, asp, ldas, wp, ldw, wsp, ldws, rp, ldr, op, ldo,
+                 0, 0), dev
 
 
-def mx_swiglu(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, codes: torch.Tensor,
-              scales: torch.Tensor, *, kernel: str | None = None) -> None:
-    """silu(a wg^T) * (a wu^T), quantised as :func:`mx_quantize` does: the input of a down projection.
-    w holds the gate's rows and then the up projection's, [2 outs, k] in e2m1 blocks; codes and scales
-    are of [rows, outs], outs a multiple of 32. The products are not rounded before."""
+def _mx_swiglu_desc(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, codes: torch.Tensor,
+                    scales: torch.Tensor) -> tuple[bytes, int]:
     entry = "th_mx_gemm"
     if len(scales.shape) != 2 or len(a_scales.shape) != 2:
         _refuse(entry, "scales are [rows, blocks]")
@@ -725,8 +716,46 @@ def mx_swiglu(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales
     ct, cp, ldc, sp, lds = _mx(codes, scales, rows, out_blocks, dev, entry, "the result's blocks")
     if wt != abi.TH_F4E2M1:
         _refuse(entry, "w must be uint8 codes of e2m1 pairs")
-    d = _pack(entry, _MXG, rows, 32 * out_blocks, blocks, at, ct, 1, 0, ap, lda, asp, ldas, wp, ldw, wsp, ldws, 0, 0, cp, ldc, sp, lds)
-    _launch(entry, d, dev, kernel)
+    return _pack(entry, _MXG, rows, 32 * out_blocks, blocks, at, ct, 1, 0, ap, lda, asp, ldas, wp, ldw, wsp, ldws, 0, 0, cp, ldc,
+                 sp, lds), dev
+
+
+def mx_gemm(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor, *,
+            residual: torch.Tensor | None = None, kernel: str | None = None) -> torch.Tensor:
+    """out[m, n] = sum_k a[m, k] w[n, k] (+ residual[m, n]): activations in e4m3 or e2m1 blocks,
+    weights in e2m1 blocks ([outs, k], one row an output column), fp32 sums, out and residual bf16 or
+    fp32 of one type. ``residual`` may be ``out``. k is whole blocks: what :func:`mx_quantize` filled up with zeros adds
+    nothing."""
+    _launch("th_mx_gemm", *_mx_gemm_desc(a, a_scales, w, w_scales, out, residual), kernel)
+    return out
+
+
+def mx_swiglu(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, codes: torch.Tensor,
+              scales: torch.Tensor, *, kernel: str | None = None) -> None:
+    """silu(a wg^T) * (a wu^T), quantised as :func:`mx_quantize` does: the input of a down projection.
+    w holds the gate's rows and then the up projection's, [2 outs, k] in e2m1 blocks; codes and scales
+    are of [rows, outs], outs a multiple of 32. The products are not rounded before."""
+    _launch("th_mx_gemm", *_mx_swiglu_desc(a, a_scales, w, w_scales, codes, scales), kernel)
+
+
+def _mx_form(desc: bytes, dev: int) -> tuple[int, bool]:
+    form = (C.c_int32 * 2)()
+    with torch.cuda.device(dev) if dev >= 0 else contextlib.nullcontext():
+        abi.check(abi.load().th_mx_gemm_form(desc, form), "th_mx_gemm_form")
+    return form[0], bool(form[1])
+
+
+def mx_gemm_form(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor, *,
+                 residual: torch.Tensor | None = None) -> tuple[int, bool]:
+    """(abi.MX_*, whether the scales are loaded byte by byte): what :func:`mx_gemm` runs for these tensors, which may
+    also be on the CPU (then for 256 compute units)."""
+    return _mx_form(*_mx_gemm_desc(a, a_scales, w, w_scales, out, residual))
+
+
+def mx_swiglu_form(a: torch.Tensor, a_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, codes: torch.Tensor,
+                   scales: torch.Tensor) -> tuple[int, bool]:
+    """The same of :func:`mx_swiglu`."""
+    return _mx_form(*_mx_swiglu_desc(a, a_scales, w, w_scales, codes, scales))
 
 
 # ----------------------------------------------------------- epilogue VM
