@@ -432,8 +432,10 @@ int th_page_copy(const th_page_copy_desc* desc, void* stream);
  * nb = ceil(cols / 32) blocks: nb scale bytes and 32 nb (e4m3) or 16 nb (e2m1)
  * code bytes; what the last block has past cols is written as zeros. Codes are
  * 16-byte aligned with row strides in whole 16 bytes; scales take any stride
- * and alignment. Strides of codes and scales are in bytes. Codes and scales that
- * a call writes share no memory with what it reads.
+ * and alignment. Strides of codes and scales are in bytes. What a call writes
+ * shares no byte with what it reads (checked, and refused), but where a tensor
+ * may be another one: then with the same rows. Rows of one tensor may lie
+ * between those of another.
  */
 
 /* x [rows, cols] to blocks: s = floor(log2(max |x|)) - emax + 127 held to 0 ..

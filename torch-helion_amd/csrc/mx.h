@@ -4,6 +4,8 @@
 
 #include "common.h"
 
+#include <algorithm>
+
 namespace th {
 
 constexpr int kMxEmaxE4M3 = 8, kMxEmaxE2M1 = 2;  // exponent of a format's largest value
@@ -95,5 +97,37 @@ __device__ __forceinline__ void mx_store8b(uint16_t* p, uint2 v) {
   *(TH_GLOBAL u2*)p = u2{v.x, v.y};
 }
 #undef TH_GLOBAL
+
+// ------------------------------------------------------------ host side
+// The bytes that a tensor of rows stands for (none without a pointer).
+struct MxSpan {
+  const void* p;
+  int64_t rows, stride, width;  // bytes; a stride is no less than the width
+};
+
+// Whether two tensors share a byte. Rows of one may lie between those of the other.
+inline bool mx_meet(const MxSpan& a, const MxSpan& b) {
+  typedef __int128 wide;  // (strides are the caller's: their products may pass 64 bits)
+  if (!a.p || !b.p || a.rows <= 0 || b.rows <= 0) return false;
+  const wide at = (wide)(uintptr_t)b.p - (wide)(uintptr_t)a.p;  // of b's first row, from a's
+  const wide sa = a.rows > 1 ? a.stride : a.width, sb = b.rows > 1 ? b.stride : b.width;
+  if (at >= (a.rows - 1) * sa + a.width || -at >= (b.rows - 1) * sb + b.width) return false;
+  auto down = [](wide x, wide y) { return x >= 0 ? x / y : -((y - 1 - x) / y); };  // floor
+  // Rows i of a and j of b meet where -b.width < at + j sb - i sa < a.width.
+  if (sa == sb)  // by i - j
+    return std::max<wide>(down(at - a.width, sa) + 1, 1 - b.rows) <= std::min<wide>(-down(-(at + b.width), sa) - 1, a.rows - 1);
+  if (a.rows > b.rows) return mx_meet(b, a);
+  const wide first = std::max<wide>(0, down(at - a.width, sa) + 1);
+  const wide last = std::min<wide>(a.rows - 1, -down(-(at + (b.rows - 1) * sb + b.width), sa) - 1);
+  for (wide i = first; i <= last; ++i)
+    if (std::max<wide>(0, down(i * sa - at - b.width, sb) + 1) <= std::min<wide>(b.rows - 1, -down(-(i * sa - at + a.width), sb) - 1))
+      return true;
+  return false;
+}
+
+// The same memory altogether, rows at the same places (in place), or none in common.
+inline bool mx_same_or_apart(const MxSpan& a, const MxSpan& b) {
+  return (a.p == b.p && (a.stride == b.stride || a.rows <= 1)) || !mx_meet(a, b);
+}
 
 }  // namespace th

@@ -281,6 +281,16 @@ static int64_t place(MxRowsK& k) {
 // 28.6, but 16384 x 4096 fp32 to e4m3 65 us instead of 60.)
 static int per_wave(int64_t units) { return units >= 2 * 8 * 4 * 256 ? 2 : 1; }
 
+static int64_t element_bytes(int dtype) { return dtype == TH_BF16 ? 2 : 4; }
+template <typename D>
+static MxSpan codes_of(const D* d, const void* codes) {
+  return {codes, d->rows, d->ld_codes, cdiv(d->cols, 32) * (d->mx_dtype == TH_F4E2M1 ? 16 : 32)};
+}
+template <typename D>
+static MxSpan scales_of(const D* d) {
+  return {d->scales, d->rows, d->ld_scales, cdiv(d->cols, 32)};
+}
+
 }  // namespace th
 
 using namespace th;
@@ -313,7 +323,9 @@ extern "C" int th_mx_quantize(const th_mx_quantize_desc* d, void* stream) {
   TH_CHECK_ARG(d->ld_x >= d->cols, "th_mx_quantize: x row stride smaller than cols");
   if (d->rows == 0) return TH_OK;
   TH_CHECK_ARG(d->x && d->codes && d->scales, "th_mx_quantize: null tensor pointer");
-  TH_CHECK_ARG(d->codes != d->x && (void*)d->scales != d->x && (void*)d->scales != d->codes,
+  const MxSpan x{d->x, d->rows, d->ld_x * element_bytes(d->x_dtype), d->cols * element_bytes(d->x_dtype)};
+  const MxSpan codes = codes_of(d, d->codes), scales = scales_of(d);
+  TH_CHECK_ARG(!mx_meet(codes, x) && !mx_meet(scales, x) && !mx_meet(scales, codes),
                "th_mx_quantize: codes and scales need memory of their own");
   TH_CHECK_READY("th_mx_quantize");
   MxRowsK k{};
@@ -343,7 +355,8 @@ extern "C" int th_mx_dequantize(const th_mx_dequantize_desc* d, void* stream) {
   TH_CHECK_ARG(d->ld_out >= d->cols, "th_mx_dequantize: out row stride smaller than cols");
   if (d->rows == 0) return TH_OK;
   TH_CHECK_ARG(d->out && d->codes && d->scales, "th_mx_dequantize: null tensor pointer");
-  TH_CHECK_ARG(d->out != d->codes && d->out != (const void*)d->scales, "th_mx_dequantize: out needs memory of its own");
+  const MxSpan out{d->out, d->rows, d->ld_out * element_bytes(d->out_dtype), d->cols * element_bytes(d->out_dtype)};
+  TH_CHECK_ARG(!mx_meet(out, codes_of(d, d->codes)) && !mx_meet(out, scales_of(d)), "th_mx_dequantize: out needs memory of its own");
   TH_CHECK_READY("th_mx_dequantize");
   MxRowsK k{};
   k.rows = d->rows; k.cols = d->cols;
@@ -381,9 +394,15 @@ extern "C" int th_mx_rmsnorm(const th_mx_rmsnorm_desc* d, void* stream) {
                "th_mx_rmsnorm: in place needs one row stride");
   if (d->rows == 0) return TH_OK;
   TH_CHECK_ARG(d->x && d->gain && d->codes && d->scales, "th_mx_rmsnorm: null tensor pointer");
-  for (const void* own : {(const void*)d->codes, (const void*)d->scales})
-    TH_CHECK_ARG(own != d->x && own != d->residual && own != d->sum_out && own != (const void*)d->gain,
+  const int64_t size = element_bytes(d->x_dtype), width = d->cols * size;
+  const MxSpan x{d->x, d->rows, d->ld_x * size, width}, residual{d->residual, d->rows, d->ld_residual * size, width};
+  const MxSpan sum{d->sum_out, d->rows, d->ld_sum_out * size, width}, gain{d->gain, 1, 0, (int64_t)d->cols * 4};
+  const MxSpan codes = codes_of(d, d->codes), scales = scales_of(d);
+  for (const MxSpan& own : {codes, scales})
+    TH_CHECK_ARG(!mx_meet(own, x) && !mx_meet(own, residual) && !mx_meet(own, sum) && !mx_meet(own, gain),
                  "th_mx_rmsnorm: codes and scales need memory of their own");
+  TH_CHECK_ARG(!mx_meet(scales, codes) && !mx_meet(sum, gain) && mx_same_or_apart(sum, x) && mx_same_or_apart(sum, residual),
+               "th_mx_rmsnorm: codes, scales and sum_out need memory of their own; sum_out may be x or residual");
   TH_CHECK_READY("th_mx_rmsnorm");
   MxNormK k{};
   k.rows = d->rows; k.cols = d->cols; k.chunks = (int)cdiv(d->cols, 32) * 4;

@@ -904,7 +904,7 @@ static int check(const th_mx_gemm_desc* d) {
     TH_CHECK_ARG(d->out_dtype == TH_BF16 || d->out_dtype == TH_F32, "th_mx_gemm: out_dtype %d unsupported", d->out_dtype);
     TH_CHECK_ARG(d->ld_out >= d->outs && (!d->residual || d->ld_residual >= d->outs),
                  "th_mx_gemm: out or residual row stride smaller than outs");
-    TH_CHECK_ARG(d->residual != d->out || d->ld_residual == d->ld_out || d->rows <= 1,
+    TH_CHECK_ARG(!d->residual || d->residual != d->out || d->ld_residual == d->ld_out || d->rows <= 1,
                  "th_mx_gemm: in place needs one row stride");
   }
   return TH_OK;
@@ -920,8 +920,26 @@ static MxGemmK operands(const th_mx_gemm_desc* d) {
   return k;
 }
 
+// What is written shares no byte with what is read; the residual may be out.
+static int check_memory(const th_mx_gemm_desc* d) {
+  const int64_t size = d->swiglu ? 1 : d->out_dtype == TH_F32 ? 4 : 2, sides = d->swiglu ? 2 : 1;
+  const MxSpan read[] = {{d->a, d->rows, d->ld_a, (int64_t)d->blocks * (d->a_dtype == TH_F4E2M1 ? 16 : 32)},
+                         {d->a_scales, d->rows, d->ld_a_scales, d->blocks},
+                         {d->w, sides * d->outs, d->ld_w, (int64_t)d->blocks * 16},
+                         {d->w_scales, sides * d->outs, d->ld_w_scales, d->blocks}};
+  const MxSpan out{d->out, d->rows, d->ld_out * size, d->swiglu && d->out_dtype == TH_F4E2M1 ? d->outs / 2 : d->outs * size};
+  const MxSpan scales{d->swiglu ? d->out_scales : nullptr, d->rows, d->ld_out_scales, d->outs / 32};
+  const MxSpan residual{d->residual, d->rows, d->ld_residual * size, d->outs * size};
+  for (const MxSpan& r : read)
+    TH_CHECK_ARG(!mx_meet(out, r) && !mx_meet(scales, r), "th_mx_gemm: the result needs memory of its own");
+  TH_CHECK_ARG(!mx_meet(out, scales) && mx_same_or_apart(out, residual),
+               "th_mx_gemm: the result needs memory of its own; a residual may be out, row for row");
+  return TH_OK;
+}
+
 extern "C" int th_mx_gemm_form(const th_mx_gemm_desc* d, int32_t* form) {
-  const int status = check(d);
+  int status = check(d);
+  if (status == TH_OK) status = check_memory(d);
   if (status != TH_OK) return status;
   TH_CHECK_ARG(form != nullptr, "th_mx_gemm_form: null pointer");
   const MxGemmK k = operands(d);
@@ -931,7 +949,7 @@ extern "C" int th_mx_gemm_form(const th_mx_gemm_desc* d, int32_t* form) {
 }
 
 extern "C" int th_mx_gemm(const th_mx_gemm_desc* d, void* stream) {
-  const int status = check(d);
+  int status = check(d);
   if (status != TH_OK || d->rows == 0) return status;
   TH_CHECK_ARG(d->a && d->a_scales && d->w && d->w_scales && d->out && (!d->swiglu || d->out_scales),
                "th_mx_gemm: null tensor pointer");
@@ -941,6 +959,8 @@ extern "C" int th_mx_gemm(const th_mx_gemm_desc* d, void* stream) {
     set_error("th_mx_gemm: th_init was not called for the current device");
     return TH_ERR_NOT_INIT;
   }
+  status = check_memory(d);
+  if (status != TH_OK) return status;
   const MxGemmK k = operands(d);
   const bool a4 = d->a_dtype == TH_F4E2M1;
   hipStream_t s = (hipStream_t)stream;
