@@ -471,7 +471,8 @@ int th_mx_dequantize(const th_mx_dequantize_desc* desc, void* stream);
 
 /* A residual's addition, the RMSNorm of the sum and its quantisation:
  *   h = x + residual in fp32, rounded to x_dtype     (residual optional: else h = x)
- *   y = h * (sum_k h^2 / cols + eps) ^ -1/2 * gain   (fp32)
+ *   y = h * (sum_k h^2 / cols + eps) ^ -1/2 * gain   (fp32; finite rows of any size,
+ *                                                     those whose squares leave fp32's range too)
  * codes, scales = the blocks of y (th_mx_quantize). sum_out (optional) gets h;
  * it may be x or residual, with their row stride.
  */

@@ -185,7 +185,6 @@ __global__ void __launch_bounds__(64 * NW) mx_rmsnorm_kernel(MxNormK p) {
   if (row >= p.rows) return;
   const T* x = (const T*)p.x + row * p.ldx;
   float v[CH][8];
-  float ss = 0.f;
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
     const int c = i * 64 * NW + tid;
@@ -219,20 +218,41 @@ __global__ void __launch_bounds__(64 * NW) mx_rmsnorm_kernel(MxNormK p) {
       mx_store8(h, c * 8, p.cols, v[i]);
     }
   }
+  // the sum of squares in units of 1 / by, the same bits in every thread
+  auto sum_squares = [&](float by) __attribute__((always_inline)) {
+    float ss = 0.f;
 #pragma unroll
-  for (int i = 0; i < CH; ++i)
+    for (int i = 0; i < CH; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss = fmaf(v[i][j], v[i][j], ss);
+      for (int j = 0; j < 8; ++j) {
+        const float x = v[i][j] * by;
+        ss = fmaf(x, x, ss);
+      }
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) ss += __shfl_xor(ss, d);
-  if constexpr (NW > 1) {
-    if ((tid & 63) == 0) part[tid >> 6] = ss;
-    __syncthreads();
-    ss = 0.f;
+    for (int d = 1; d < 64; d <<= 1) ss += __shfl_xor(ss, d);
+    if constexpr (NW > 1) {
+      if ((tid & 63) == 0) part[tid >> 6] = ss;
+      __syncthreads();
+      ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < NW; ++i) ss += part[i];
+      for (int i = 0; i < NW; ++i) ss += part[i];
+    }
+    return ss;
+  };
+  const float mean = sum_squares(1.f) * p.inv_n + p.eps;
+  float rs = rsqrtf(mean);
+  // Squares past fp32's range (of values from 2^56 on), or so far below it that they lose bits (and eps with them): the sum
+  // again in units of 2^80 or 2^-100, in which it is 2^112 or 2^96 at most. Half of the unit's power then goes to the
+  // values and half to the root, so that neither leaves the range.
+  if (mean == __uint_as_float(0x7f800000u) || mean < 0x1p-120f) {
+    const float half = mean < 1.f ? 0x1p50f : 0x1p-40f;
+    if constexpr (NW > 1) __syncthreads();  // every wave has read the parts
+    rs = rsqrtf(sum_squares(half * half) * p.inv_n + p.eps * (half * half) * (half * half)) * half;
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] *= half;
   }
-  const float rs = rsqrtf(ss * p.inv_n + p.eps);
   uint8_t* codes = p.codes + row * p.ldc;
   uint8_t* scales = p.scales + row * p.lds;
 #pragma unroll
