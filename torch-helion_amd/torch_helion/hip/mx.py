@@ -15,12 +15,16 @@ from .paged import PagedDecodeBlock
 
 class MxDecodeBlock(PagedDecodeBlock):
     """``PagedDecodeBlock`` with weights in e2m1 blocks of 32 along k; ``bits`` 8 (e4m3) or 4 (e2m1) are the
-    activations' elements. intermediate is a multiple of 32. ``effective_weights`` are the values that the
-    codes stand for; there is no ``out32``, the sums are rounded to the bf16 stream once."""
+    activations' elements. intermediate is a multiple of 32, hidden at most 65536. ``effective_weights`` are the
+    values that the codes stand for; there is no ``out32``, the sums are rounded to the bf16 stream once.
+    ``fold_gain`` makes no difference: a norm always applies its gain as it quantises."""
 
     def __init__(self, state_dict: dict[str, torch.Tensor], *, bits: int = 8, **options) -> None:
         if bits not in (4, 8):
             raise abi.HipBackendError("MxDecodeBlock", abi.TH_ERR_INVALID, f"activations of {bits} bits; 4 or 8")
+        if options.get("intermediate", 0) % 32 or options.get("hidden", 0) > 65536:
+            raise abi.HipBackendError("MxDecodeBlock", abi.TH_ERR_INVALID, f"intermediate {options.get('intermediate')} must be whole "
+                                      f"blocks of 32, hidden {options.get('hidden')} at most 65536")
         self.bits = bits
         super().__init__(state_dict, **options)
 
