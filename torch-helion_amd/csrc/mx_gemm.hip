@@ -11,13 +11,13 @@
 // 2^(E - 13). Of e2m1 activations nothing does. Of e4m3 ones E <= 8 + 2 and bits reach down to 2^-10, so that the values of 2
 // and more and those below are multiplied apart, two products for one: of the former E <= 10 and the last bit is 2^-3, of
 // the latter E <= 2 and 2^-10, and nothing is cut. The sums are fp32. (With one product 16384 x 4096 x 14336 took 690 us
-// for 1115, 64 rows 15.2 for 15.9, and of the SwiGLU's e4m3 codes one in 18000 fell on the other side of a rounding. bf16
+// for 1100, 64 rows 15.2 for 15.9, and of the SwiGLU's e4m3 codes one in 18000 fell on the other side of a rounding. bf16
 // products have a quarter of the rate, and both operands to convert.)
 // (The 32x32x64 form has the same rate on zeros, and 3.98 against 4.73 PFLOP/s on random values.)
 //
 // What bounds it: with few rows the weights (64 x 4096 x 14336: 31 MB, 6 us at the 5.2 TB/s of a copy; 15.9 us, since each
 // CU takes in 40 to 50 GB/s of activations and weights), with many the matrix cores and what feeds them:
-// 16384 x 4096 x 14336 1115 us (1.73 PFLOP/s, of two products each 3.45), SwiGLU of 8192 x 14336 x 4096 1115 (1.73); 6001 x
+// 16384 x 4096 x 14336 1100 us (1.75 PFLOP/s, of two products each 3.5), SwiGLU of 8192 x 14336 x 4096 1110 (1.73); 6001 x
 // 14336 x 4096 of e2m1 235 us (3.0). Of the first the matrix cores are busy for 79 % of the cycles, at 2.15 GHz.
 //
 // Operand layout of v_mfma_scale_f32_16x16x128_f8f6f4: lane l supplies row l % 16;
@@ -218,8 +218,8 @@ __device__ __forceinline__ void mx_lds_order() {
 
 // Output tile of a workgroup: XCD x (workgroups x, x + 8, ...) takes one contiguous range of
 // tiles, four tile rows at a time: of the lines that its 32 workgroups load a stage, those of a
-// count twice those of w (e4m3), so that 4 x 8 tiles load fewest (16384 x 4096 x 14336: 720 us, with
-// eight tile rows 733, with two 729).
+// count twice those of w (e4m3), so that 4 x 8 tiles load fewest (16384 x 4096 x 14336 with one product for all of an
+// e4m3 value: 720 us, with eight tile rows 733, with two 729).
 __device__ __forceinline__ void mx_tile_of(int L, int tiles_m, int tiles_n, int& tm, int& tn) {
   const int all = tiles_m * tiles_n, q = all >> 3, r = all & 7, x = L & 7;
   const int id = x * q + min(x, r) + (L >> 3);
@@ -235,7 +235,8 @@ __device__ __forceinline__ void mx_tile_of(int L, int tiles_m, int tiles_n, int&
 // whose rows an operand takes as 8 (i / 4) + i % 4). A read of 16 bytes a lane goes 16 lanes at a time, lanes 0 .. 3, 12 .. 15
 // and 20 .. 27 first, then 4 .. 11, 16 .. 19 and 28 .. 31 (found from the conflicts counted): each such sixteen hits
 // every one of 64 banks once, in tiles and rings. (Swizzles made for sixteen lanes in a row cost four cycles a read more:
-// 155 million LDS cycles of 16384 x 4096 x 14336 became 96, its time stayed the same.)
+// of 16384 x 4096 x 14336, then in waves of 4 x 8 subtiles, 155 million LDS cycles for 96 in the same time. In waves of 2 x 16
+// it takes 136 million, 29 of them conflicts.)
 __device__ __forceinline__ int mx_sw8(int r) { return (r >> 1) & 7; }
 __device__ __forceinline__ int mx_sw4(int p) { return (p & 2) ^ (((p >> 2) & 1) * 3); }
 __device__ __forceinline__ int mx_sww(int p) { return (p >> 1) & 2; }
@@ -251,9 +252,9 @@ struct MxTile {
   // ODD: a stage's scales lie behind it, a dword each. Else:
   static constexpr int STAGE = ABYTES + WBYTES + (ODD ? 16 * (BM + BN) : 0);
   // scales: sets of 8 bytes a row, those of two stages; half a set is loaded with each stage, the set after the stage's
-  // own, over one whose last stage has been read then. (A dword a row and stage: 902 us instead of 833, since each
-  // row is a line of its own; none at all, in a copy: 798. Sets of 16 and 32 bytes were slower, 750 against 716, for
-  // the addresses that they take.)
+  // own, over one whose last stage has been read then. (16384 x 4096 x 14336 with one product for all of an e4m3 value: a
+  // dword a row and stage 902 us instead of 833, since each row is a line of its own; none at all, in a copy, 798. Sets of
+  // 16 and 32 bytes were slower, 750 against 716, for the addresses that they take.)
   static constexpr int SETS = ODD ? 0 : (STAGES + 4) / 2, SET = 8 * (BM + BN), SCALES = STAGES * STAGE;
   static constexpr int LDS = SCALES + SETS * SET;
   static constexpr int PA = ABYTES / 1024, PW = WBYTES / 1024, SP = (BM + BN) / (ODD ? 16 : 64);  // loads: 1 KiB, 32 rows of scales (ODD: 16)
@@ -448,8 +449,8 @@ __global__ void __launch_bounds__(64 * WM * WN) mx_gemm_tile_kernel(MxGemmK p, i
   // has the stage in registers, and while that group is multiplied the stage's place is refilled, the next stage's first
   // group is read, and its activations. All of that goes between the products: the two waves of a SIMD meet at the
   // barrier, and what stands before their next products leaves the matrix cores idle. e4m3 activations are split there too,
-  // once a stage for all columns: so a wave has few row subtiles and many column subtiles (256 x 256: 2 and 16, 1115 us; 4 and
-  // 8, split for every group, 1196).
+  // once a stage for all columns: so a wave has few row subtiles and many column subtiles (256 x 256: 2 and 16;
+  // with 4 and 8, split for every group, 1196 us for 1132 when the split was two instructions longer).
   constexpr int H = T::GROUP;
   int st = 0;
   auto stage = [&](int kt) __attribute__((always_inline)) {
@@ -665,7 +666,7 @@ static void launch_tile(const MxGemmK& k, hipStream_t s) {
 // 32 columns (with SWIGLU of the gate and of the up projection) of up to 32 rows a workgroup; the stages
 // of k (128 values) are dealt out to its eight waves, each with a ring of STAGES stages of its own in LDS:
 // no wave waits for another before the sums are added, and all of a ring's loads are in flight (1 x 6144 x 4096
-// 4.9 us, 2.7 TB/s of weights; 64 x 4096 x 14336 15.4 us, where operands held in registers took 42).
+// 5.9 us, 2.3 TB/s of weights; 64 x 4096 x 14336 15.9 us, where operands held in registers took 42).
 // AP: pieces of a stage's activations (8 rows of e4m3, 16 of e2m1). ODD: as above.
 template <bool A4, bool SWIGLU, bool ODD, int AP, int STAGES>
 __global__ void __launch_bounds__(512) mx_gemm_ring_kernel(MxGemmK p) {
